@@ -55,6 +55,15 @@ SIGNATURES = {
     "cmb_gemm_set_sm_die_map": (_i, [_p, _i]),
     "cmb_mma_rate": (_i, [_i, _i, _i, _p, _p, _p, _p]),
     "cmb_quantize_e4m3": (_i, [_p, _sz, _p, _p, _p]),
+    "cmb_quantize_e4m3_block128": (_i, [_p, _i, _i, _i, _sz, _i, _p, _sz, _p, _sz, _p, _sz, _p,
+                                        _sz, _p]),
+    "cmb_gemm_e4m3_block128": (_i, [_p, _sz, _p, _sz, _p, _sz, _p, _sz, _i, _p, _sz, _i, _i, _i,
+                                    _i, _p, _p]),
+    "cmb_rmsnorm_e4m3_block128": (_i, [_p, _sz, _p, _sz, _i, _p, _i, _f, _i, _i, _p, _sz, _p, _sz,
+                                       _p, _sz, _p, _sz, _p, _p]),
+    "cmb_rmsnorm_backward_workspace_bytes": (_sz, [_i, _i]),
+    "cmb_rmsnorm_backward": (_i, [_p, _sz, _p, _sz, _p, _sz, _i, _p, _i, _p, _i, _i, _p, _sz, _p,
+                                  _p, _sz, _p]),
     "cmb_mma_sync_latency": (_i, [_i, _i, _p, _p, _p]),
     "cmb_mma_sync_throughput": (_i, [_i, _i, _i, _i, _p, _p]),
     "cmb_p2p_alloc": (_i, [_sz, _p]),

@@ -1,0 +1,186 @@
+// block128.cuh — the block-scaled e4m3 form shared by the quantiser, the
+// RMS norm and the GEMM: one E8M0 scale byte for each block of 128 values
+// (or 128 x 128), and 8-value chunks of bf16 or fp32 rows.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+
+#include "cmb_device.cuh"
+
+namespace cmb {
+namespace b128 {
+
+constexpr int kBlock = 128;
+constexpr float kMaxFinite = 3.40282346638528859811704183484516925e+38f;
+
+__host__ __device__ constexpr int groups_of(int n) { return (n + kBlock - 1) / kBlock; }
+
+// |x| where x is finite, 0 where it is not: what a block's scale is taken from.
+__device__ __forceinline__ float finite_magnitude(float x) {
+  const float a = fabsf(x);
+  return a <= kMaxFinite ? a : 0.0f;
+}
+
+// E8M0 byte of the smallest power of two s with amax / s <= 448.  With amax =
+// 1.m * 2^(E - 127) and 448 = 1.75 * 2^8 that is 2^(E - 127 - 8), or twice
+// that where 1.m > 1.75; integers on the bits, so every path (quantiser,
+// norm, host) agrees on a block that ends exactly at 448 * 2^n.  Under
+// 2^-127 there is no E8M0 value: those blocks keep byte 0 and lose nothing,
+// since amax / 2^-127 is then under 448.
+__device__ __forceinline__ uint32_t scale_byte(float amax) {
+  if (amax == 0.0f) return 127u;
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return static_cast<uint32_t>(max(e, 0));
+}
+
+// 2^(127 - byte), the exact reciprocal of a scale that scale_byte made (its
+// bytes reach 247, so the result is a normal number).
+__device__ __forceinline__ float scale_reciprocal(uint32_t byte) {
+  return __uint_as_float((254u - byte) << 23);
+}
+
+// Two values to e4m3 (nearest even), `lo` in the low byte.  The scale keeps
+// finite values within 448, so saturation only ever meets infinities; those
+// become NaN, as NaN does.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint32_t v = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+  if (!(fabsf(lo) <= kMaxFinite)) v = (v & 0xFF00u) | 0x7Fu;
+  if (!(fabsf(hi) <= kMaxFinite)) v = (v & 0x00FFu) | 0x7F00u;
+  return v;
+}
+
+// 8 values times `inv` as 8 e4m3 bytes.
+__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
+  uint2 q;
+  q.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
+  q.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
+  return q;
+}
+
+// ------------------------------------------------- rows of bf16 or fp32
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// 8 consecutive elements as they lie in memory.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<__nv_bfloat16> {
+  uint4 a;
+};
+template <>
+struct Raw8<float> {
+  uint4 a, b;
+};
+
+__device__ __forceinline__ Raw8<__nv_bfloat16> load8(const __nv_bfloat16 *p) {
+  return {*reinterpret_cast<const uint4 *>(p)};
+}
+__device__ __forceinline__ Raw8<float> load8(const float *p) {
+  return {reinterpret_cast<const uint4 *>(p)[0], reinterpret_cast<const uint4 *>(p)[1]};
+}
+
+__device__ __forceinline__ void unpack(const Raw8<__nv_bfloat16> &r, float (&v)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const Raw8<float> &r, float (&v)[8]) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+}
+
+__device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Rounded (nearest even) to the type of the row.
+__device__ __forceinline__ void pack(const float (&v)[8], Raw8<__nv_bfloat16> &r) {
+  r.a = make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]),
+                   bf16x2_bits(v[6], v[7]));
+}
+__device__ __forceinline__ void pack(const float (&v)[8], Raw8<float> &r) {
+  r.a = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                   __float_as_uint(v[3]));
+  r.b = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]),
+                   __float_as_uint(v[7]));
+}
+
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const Raw8<__nv_bfloat16> &r) {
+  *reinterpret_cast<uint4 *>(p) = r.a;
+}
+__device__ __forceinline__ void store8(float *p, const Raw8<float> &r) {
+  reinterpret_cast<uint4 *>(p)[0] = r.a;
+  reinterpret_cast<uint4 *>(p)[1] = r.b;
+}
+
+// Elements [0, n) of the 8 at p, zeros behind them; whole aligned chunks in
+// one or two 16-byte loads.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_edge(const T *p, int n, bool aligned) {
+  if (aligned && n >= 8) return load8(p);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.0f;
+  Raw8<T> r;
+  pack(v, r);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8_edge(T *p, const Raw8<T> &r, int n, bool aligned) {
+  if (aligned && n >= 8) {
+    store8(p, r);
+    return;
+  }
+  float v[8];
+  unpack(r, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = from_float<T>(v[i]);
+}
+
+// 8 bytes, or the first n of them.
+__device__ __forceinline__ void store_bytes(uint8_t *p, uint2 q, int n, bool aligned) {
+  if (aligned && n >= 8) {
+    *reinterpret_cast<uint2 *>(p) = q;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+}
+
+// ------------------------------------------------------------ host checks
+
+inline bool aligned_to(const void *p, size_t pitch_bytes, size_t to) {
+  return (reinterpret_cast<uintptr_t>(p) % to) == 0 && pitch_bytes % to == 0;
+}
+
+}  // namespace b128
+}  // namespace cmb

@@ -272,6 +272,90 @@ int cmb_mma_rate(int fp8, int iters, int ctas, float *out, uint64_t *cycles, int
 int cmb_quantize_e4m3(const uint16_t *src_bf16, size_t n, uint8_t *dst, float *scale_out,
                       cmb_stream_t stream);
 
+/* --- block-scaled e4m3: what a linear layer in 8 bits calls (no reference
+ *     counterpart: the reference's FP8 probes have no operands in memory) --- */
+
+/* Element types of the operands below. */
+typedef enum { CMB_BF16 = 0, CMB_F32 = 1 } cmb_dtype;
+
+/* A matrix in this form is rows x cols e4m3 bytes (row-major, `ld` bytes
+ * from row to row) and one scale byte for each block of block_rows x 128
+ * values: scale[(r / block_rows) * ld_scale + c / 128], the last block of a
+ * row or column cut short.  A scale byte s is E8M0, the power of two
+ * 2^(s - 127) (255 is NaN); a value is e4m3 * 2^(s - 127).  block_rows is 1
+ * (activations and gradients) or 128 (weights).
+ * For a block whose largest finite magnitude is a > 0, the quantisers take
+ * the smallest power of two with a / 2^(s - 127) <= 448 (but not under
+ * 2^-127), for a block of zeros 1; each value is divided by it, exactly, and
+ * rounded once to the nearest e4m3 (ties to even).  NaN and infinities
+ * become NaN (0x7F): an overflow shows in the product and leaves the rest of
+ * its block alone. */
+
+/* Quantises src (rows x cols of src_type, ld_src elements from row to row)
+ * and, in the same read, its transpose: dst, scale = the form above of src;
+ * dst_t, scale_t = the form above of src^T (cols x rows, blocks of 128 source
+ * rows), which is what the products of a backward pass read.  Either pair
+ * may be NULL.  rows = 0 or cols = 0 writes nothing.  The outputs must not
+ * overlap the input or one another.  Bytes between the end of a row and the
+ * next one's start are left as they are. */
+int cmb_quantize_e4m3_block128(const void *src, int src_type, int rows, int cols, size_t ld_src,
+                               int block_rows, uint8_t *dst, size_t ld_dst, uint8_t *scale,
+                               size_t ld_scale, uint8_t *dst_t, size_t ld_dst_t, uint8_t *scale_t,
+                               size_t ld_scale_t, cmb_stream_t stream);
+
+/* C[M x N] (c_type, row-major, ldc elements from row to row) = A * B^T for
+ * A[M x K] with blocks of 1 x 128 and B[N x K] with blocks of block_rows_b x
+ * 128, in the form above; products and sums in fp32, rounded once for a bf16
+ * C.  A linear layer's forward pass has A = activations, B = weights
+ * (block_rows_b 128); its input gradient B = the transposed weights; its
+ * weight gradient A and B both transposed, block_rows_b 1, K = tokens.
+ * M or N = 0 writes nothing; K = 0 writes zeros.  A and B: 16-byte aligned,
+ * lda and ldb multiples of 16.  *status (device, may be NULL) is not cleared:
+ * it keeps the first CMB_ERR_TIMEOUT of any call since the caller zeroed it,
+ * so a program reads it once for many products. */
+int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_t *scale_a, size_t ld_scale_a,
+                           const uint8_t *B, size_t ldb, const uint8_t *scale_b, size_t ld_scale_b,
+                           int block_rows_b, void *C, size_t ldc, int c_type, int M, int N, int K,
+                           int *status, cmb_stream_t stream);
+
+/* Root-mean-square norm with the residual's addition and an e4m3 output:
+ *   h = x + residual (rounded to `type`; h = x where residual is NULL)
+ *   rstd = (mean_c h^2 + eps)^(-1/2);  y = h * rstd * weight  (fp32)
+ *   q, scale = y in the form above with blocks of 1 x 128
+ * for each of `rows` rows of cols (<= CMB_RMSNORM_MAX_COLS) values.  x,
+ * residual, h and y have `type`, weight (cols values) weight_type; ld_* in
+ * elements (bytes for q and scale).  h is written where residual is given
+ * (h may be x or residual, element for element); y (the same y rounded to
+ * `type`, for a weight gradient), rstd (fp32, one for each row) and the pair
+ * q, scale may be NULL.  rows = 0 writes nothing. */
+#define CMB_RMSNORM_MAX_COLS 32768
+int cmb_rmsnorm_e4m3_block128(const void *x, size_t ld_x, const void *residual, size_t ld_residual,
+                              int type, const void *weight, int weight_type, float eps, int rows,
+                              int cols, void *h, size_t ld_h, void *y, size_t ld_y, uint8_t *q,
+                              size_t ld_q, uint8_t *scale, size_t ld_scale, float *rstd,
+                              cmb_stream_t stream);
+
+/* Workspace bytes cmb_rmsnorm_backward needs for its weight gradient. */
+size_t cmb_rmsnorm_backward_workspace_bytes(int rows, int cols);
+/* Gradients of that norm, y's own rounding to 8 bits passed over: with
+ * g = dy * weight,
+ *   dx = rstd * (g - h * rstd^2 * mean_c(g * h)) + dh
+ *   dweight[c] = sum_r dy * h * rstd   (fp32, in a fixed order)
+ * h and rstd are the forward pass's (h = x where it had no residual).  dh is
+ * the gradient that reaches h past the norm (NULL: none); with a residual,
+ * dx is the gradient of x and of the residual alike.  dy, h, dh and dx have
+ * `type`; dx may be dy or dh, element for element.  dweight may be NULL, and
+ * workspace with it; otherwise workspace is
+ * cmb_rmsnorm_backward_workspace_bytes(rows, cols) bytes of device memory,
+ * 16-byte aligned, that need no initialisation; two calls whose work
+ * overlaps on the GPU need separate workspaces.  rows = 0 sets dweight to
+ * zeros. */
+int cmb_rmsnorm_backward(const void *dy, size_t ld_dy, const void *h, size_t ld_h, const void *dh,
+                         size_t ld_dh, int type, const void *weight, int weight_type,
+                         const float *rstd, int rows, int cols, void *dx, size_t ld_dx,
+                         float *dweight, void *workspace, size_t workspace_bytes,
+                         cmb_stream_t stream);
+
 /* --- die-aware tile order for the GEMMs (no reference counterpart: the
  *     reference's tensor probes read no memory) ---------------------------- */
 
