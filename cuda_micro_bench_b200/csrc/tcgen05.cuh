@@ -96,7 +96,62 @@ __host__ __device__ constexpr uint32_t instr_desc() {
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Shared-memory descriptor of 32 rows of 16 bytes, 8-row (128-byte) core
+// matrices one behind the other, no swizzle: what a 32x128b copy reads.
+__device__ __forceinline__ uint64_t rows16_desc(uint32_t smem_addr) {
+  return (static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu)) | (1ull << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+}
+
+// Instruction descriptor of the block-scaled e4m3 MMA (kind::mxf8f6f4), both
+// operands K-major, E8M0 scales, fp32 accumulate: 4-5 byte of B's scale word,
+// 7-9 / 10-12 formats (0 = e4m3), 17-22 N >> 3, 23 scale format (1 = E8M0),
+// 24-28 M >> 4, 29-30 byte of A's scale word.
+__device__ __forceinline__ uint32_t instr_desc_block_scaled(int m, int n, uint32_t sf) {
+  return (sf << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 4) << 24) | (sf << 29);
+}
+
 // ---------------------------------------------------------------- MMA
+
+// D[tmem] (+)= (A * scales of A's rows) * (B * scales of B's rows)^T for 32
+// bytes of K: the scales lie in TMEM, row r's word at lane r % 32 (repeated
+// in each quarter), column r / 32; the instruction descriptor names the byte.
+template <int CG>
+__device__ __forceinline__ void mma_block_scaled(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t sfa_tmem,
+                                                 uint32_t sfb_tmem, uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{ .reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X"
+        " [%0], %1, %2, %3, [%5], [%6], p; }" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+        : "memory");
+  else
+    asm volatile(
+        "{ .reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X"
+        " [%0], %1, %2, %3, [%5], [%6], p; }" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+        : "memory");
+}
+
+// Copies 32 rows of 16 bytes of shared memory to 4 TMEM columns, lane r = row
+// r, repeated in all four lane quarters.  Issued by one thread; a later MMA
+// of the same thread sees it.  cta_group::2 copies in both CTAs of the pair,
+// each from its own shared memory.
+template <int CG>
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+}
 
 // D[tmem] (+)= A[smem] * B[smem]^T; issued by one thread.
 template <int CG, bool kFp8>
@@ -161,6 +216,18 @@ __device__ __forceinline__ void ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32])
         "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
         "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
         "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// The same for 16 columns.
+__device__ __forceinline__ void ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
