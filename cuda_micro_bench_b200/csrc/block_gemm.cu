@@ -12,16 +12,22 @@
 //
 // The MMA's 128-row side is B (the weights) and its N side is A (the
 // tokens): C^T = B * A^T.  A tile then takes as many tokens as there are, in
-// steps of 16, with nothing padded to 128 of them, and a lane of the
+// steps of 16 or 32, with nothing padded to 128 of them, and a lane of the
 // accumulator is a column of C, so a warp stores 32 neighbouring values of
 // one row of C at any alignment.
 //
-// Scales travel apart from the values: a warp gathers the scale bytes of
-// four K blocks (one 32-bit word for each row) into shared memory, tcgen05.cp
-// takes them to TMEM, and the instruction descriptor of each MMA names the
-// byte of the word its K block is.  Two buffers of words: the gather of four
-// K blocks ahead waits for the MMAs of the last four but one.
+// Scales travel apart from the values: a warp gathers the scale bytes of 16 K
+// blocks of every row into shared memory, as words of four; for each four K
+// blocks tcgen05.cp takes the words to TMEM, and the instruction descriptor of
+// each MMA names the byte of the word its K block is.  Both places have two
+// buffers.
+//
+// Two kernels: k_gemm_pair for many tokens (tensor core and L2 delivery
+// bound), k_gemm_split for few (bound by reading the weights once).
 #include <cuda.h>
+
+#include <cmath>
+#include <mutex>
 
 #include "block128.cuh"
 #include "cmb_host.h"
@@ -44,44 +50,162 @@ struct Args {
   void *C;
   int w_rows, t_rows, K, groups;
   int w_shift;               // 7 where B has blocks of 128 x 128, else 0
-  bool w_words, t_words;     // scale rows can be read in aligned words
+  bool w_vec, t_vec;     // scale rows can be read 16 bytes at a time
   bool bf16;                 // C's type
   int n;                     // token rows of an MMA
   int stages;
-  int split;                 // CTAs that share a tile's K
+  int split;                 // CTAs that share a tile's K (k_gemm_split)
+  int tmem_cols;             // TMEM columns to allocate (k_gemm_split)
   int *status;
 };
 
 constexpr int kMaxStages = 12;
 constexpr int kWBytes = 128 * 128;      // a K block of 128 weight rows
 constexpr int kScaleSlot = 512 + 1024;  // scale words of 128 weight rows and 256 token rows
+constexpr int kSplitSlot = 512 + 512;   // the same with 128 token rows
 constexpr int kScaleCol = 480;          // TMEM columns of the scales: 2 x 4 and 2 x 8
 constexpr size_t kSmemMost = 227 * 1024 - 1024;  // less what is static
+constexpr size_t kSmemHalf = 112 * 1024;         // two CTAs a SM
+constexpr int kSplitThreads = 256;
 
-// The scale bytes of K blocks 4b .. 4b + 3 of a row, 0 where there is none.
-__device__ __forceinline__ uint32_t scale_word(const uint8_t *scale, size_t ld, int row, int rows,
-                                               int shift, int b, int groups, bool words) {
-  if (row >= rows) return 0u;
-  const uint8_t *p = scale + static_cast<size_t>(row >> shift) * ld + 4 * b;
-  const int n = groups - 4 * b;
-  if (words && n >= 4) return __ldg(reinterpret_cast<const uint32_t *>(p));
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) w |= static_cast<uint32_t>(__ldg(p + i)) << (8 * i);
-  return w;
-}
-
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint32_t (&v)[4]) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
-               "r"(v[2]), "r"(v[3])
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// The scale bytes of K blocks 16 s .. 16 s + 15 of 4 U rows, each 32 behind the
+// one before; rows behind the last give the last one's (the values there are
+// zeros), K blocks behind the last anything, which no MMA reads.  32 lanes read
+// 32 rows, so each load is 32 sectors: one for 16 K blocks, all in flight at
+// once.  With a word for 4 K blocks and load the gather, not the tensor core,
+// set the pace (1.0 us a K block of the 480-token tile).
+template <int U>
+__device__ __forceinline__ void scale_pieces(uint4 (&v)[4 * U], const uint8_t *scale, size_t ld,
+                                             int row, int rows, int shift, int s, int groups,
+                                             bool vec) {
+  const uint8_t *p[4 * U];
+#pragma unroll
+  for (int c = 0; c < 4 * U; ++c)
+    p[c] = scale + static_cast<size_t>(min(row + 32 * c, rows - 1) >> shift) * ld + 16 * s;
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < 4 * U; ++c) v[c] = __ldg(reinterpret_cast<const uint4 *>(p[c]));
+  } else {
+    const int last = groups - 1 - 16 * s;
+#pragma unroll
+    for (int c = 0; c < 4 * U; ++c) v[c] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int i = 0; i <= min(last, 15); ++i) {
+      uint32_t byte[4 * U];
+#pragma unroll
+      for (int c = 0; c < 4 * U; ++c) byte[c] = __ldg(p[c] + i);
+      const int word = i >> 2, at = 8 * (i & 3);
+#pragma unroll
+      for (int c = 0; c < 4 * U; ++c) {
+        v[c].x |= word == 0 ? byte[c] << at : 0u;
+        v[c].y |= word == 1 ? byte[c] << at : 0u;
+        v[c].z |= word == 2 ? byte[c] << at : 0u;
+        v[c].w |= word == 3 ? byte[c] << at : 0u;
+      }
+    }
+  }
+}
+
+// Four words of each of U times 128 rows, for 4 times 4 K blocks, where the
+// copies to TMEM look for them: lane r's four words are those of rows r, 32 +
+// r, 64 + r and 96 + r.
+template <int U>
+__device__ __forceinline__ void put_pieces(uint32_t at, uint32_t slot_bytes,
+                                           const uint4 (&v)[4 * U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint4 *q = v + 4 * u;
+    st_shared_v4(at + 512 * u, q[0].x, q[1].x, q[2].x, q[3].x);
+    st_shared_v4(at + 512 * u + slot_bytes, q[0].y, q[1].y, q[2].y, q[3].y);
+    st_shared_v4(at + 512 * u + 2 * slot_bytes, q[0].z, q[1].z, q[2].z, q[3].z);
+    st_shared_v4(at + 512 * u + 3 * slot_bytes, q[0].w, q[1].w, q[2].w, q[3].w);
+  }
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
+}
+
+// The value of lane 0, which the compiler then knows to be the same in every
+// lane: the roles' branches, and the operands that MMAs and loads take from
+// uniform registers, stay out of the vector registers.
+__device__ __forceinline__ int uniform(uint32_t v) {
+  return static_cast<int>(__shfl_sync(0xffffffffu, v, 0));
+}
+
+// The rest of a wait whose phase was not complete at once: false after
+// kWaitLimitNs, or once another role of the CTA has given up.
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag,
+                                       int *status) {
+  const uint64_t deadline = dev::globaltimer() + dev::kWaitLimitNs;
+#pragma unroll 1
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (__all_sync(0xffffffffu, dev::mbar_try_wait_cluster_acq(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0 || dev::globaltimer() > deadline)) break;
+  }
+  dev::report_status(status, CMB_ERR_TIMEOUT);
+  *abort_flag = 1;
+  return false;
+}
+
+// Waits of the whole warp.  Out of line from the second try on: with the whole
+// bounded loop and a look at the abort flag in its path, a wait that is
+// already over cost the issuing warp ~290 cycles, half a K block's MMAs.
+struct Waiter {
+  volatile int *abort_flag;
+  int *status;
+  __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const {
+    const uint32_t b = dev::smem_addr(bar);
+    return __all_sync(0xffffffffu, dev::mbar_try_wait(b, parity)) ||
+           wait_long(b, parity, abort_flag, status);
+  }
+  // For a barrier that threads of the other CTA arrive on.
+  __device__ __forceinline__ bool of_pair(uint64_t *bar, uint32_t parity) const {
+    const uint32_t b = dev::smem_addr(bar);
+    return __all_sync(0xffffffffu, dev::mbar_try_wait_cluster_acq(b, parity)) ||
+           wait_long(b, parity, abort_flag, status);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_as(T *p, float v) {
+  *p = b128::from_float<T>(v);
+}
+
+// N accumulator columns, rows t .. t + N - 1 of C at column w, of which the
+// first `rows` are there: 32 lanes write 32 neighbours of each row.
+template <typename T, int N>
+__device__ __forceinline__ void store_columns(const Args &g, int t, int w, int rows,
+                                              const uint32_t *r) {
+  T *p = static_cast<T *>(g.C) + static_cast<size_t>(t) * g.ldc + w;
+  if (rows >= N) {
+#pragma unroll
+    for (int c = 0; c < N; ++c, p += g.ldc) store_as(p, __uint_as_float(r[c]));
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c, p += g.ldc)
+      if (c < rows) store_as(p, __uint_as_float(r[c]));
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void store_columns(const Args &g, int t, int w, const uint32_t *r) {
+  if (w >= g.w_rows) return;
+  if (g.bf16) store_columns<__nv_bfloat16, N>(g, t, w, g.t_rows - t, r);
+  else store_columns<float, N>(g, t, w, g.t_rows - t, r);
 }
 
 __device__ __forceinline__ void store_c(const Args &g, int t, int w, float v) {
@@ -94,18 +218,18 @@ __device__ __forceinline__ void store_c(const Args &g, int t, int w, float v) {
 // the `split` CTAs of a tile are one cluster and add their parts, in order,
 // through distributed shared memory.
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-7 accumulator
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(kSplitThreads, 2)
     k_gemm_split(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t,
                  const Args g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
-  __shared__ __align__(8) uint64_t sfull[2], sfree[2], done;
+  __shared__ __align__(8) uint64_t sfull[2], sfree[2], bdone[2], done;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int stage_bytes = kWBytes + g.n * 128;
   uint8_t *scales = ring + (size_t)g.stages * stage_bytes;
   const int part = blockIdx.x % g.split, tile = blockIdx.x / g.split;
@@ -122,6 +246,7 @@ __global__ void __launch_bounds__(256, 1)
     for (int s = 0; s < 2; ++s) {
       dev::mbar_init(dev::smem_addr(&sfull[s]), 1);
       dev::mbar_init(dev::smem_addr(&sfree[s]), 1);
+      dev::mbar_init(dev::smem_addr(&bdone[s]), 1);
     }
     dev::mbar_init(dev::smem_addr(&done), 1);
     abort_flag = 0;
@@ -130,106 +255,104 @@ __global__ void __launch_bounds__(256, 1)
     dev::tma_prefetch_desc(&tm_t);
   }
   if (warp == 1) {
-    tc::tmem_alloc<1>(dev::smem_addr(&tmem_holder), 512);
+    tc::tmem_alloc<1>(dev::smem_addr(&tmem_holder), g.tmem_cols);
     tc::tmem_relinquish<1>();
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_holder;
-  // A wait that gives up reports and makes every role leave; false once one has.
-  const auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (dev::mbar_wait_bounded(dev::smem_addr(bar), parity) &&
-        *static_cast<volatile int *>(&abort_flag) == 0)
-      return true;
-    dev::report_status(g.status, CMB_ERR_TIMEOUT);
-    atomicExch(&abort_flag, 1);
-    return false;
-  };
+  const uint32_t tmem = uniform(tmem_holder);
+  const Waiter wait{&abort_flag, g.status};
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
 
+  // Warps 0 and 1 stay whole and elect a lane for each issue: their operands
+  // are then warp-uniform, which the tensor core's and TMA's instructions need.
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0, kb = kb0;
-      uint32_t ph = 0;
-      for (; kb < kb1; ++kb) {
-        if (!wait(&empty[s], ph ^ 1)) break;
-        uint8_t *w = ring + (size_t)s * stage_bytes;
-        const uint32_t bar = dev::smem_addr(&full[s]);
+    int s = 0, kb = kb0;
+    uint32_t ph = 0;
+    for (; kb < kb1; ++kb) {
+      if (!wait(&empty[s], ph ^ 1)) break;
+      uint8_t *w = ring + (size_t)s * stage_bytes;
+      const uint32_t bar = dev::smem_addr(&full[s]);
+      if (dev::elect_one()) {
         dev::mbar_arrive_expect_tx(bar, stage_bytes);
         dev::tma_load_2d(dev::smem_addr(w), &tm_w, kb * kBlock, w0, bar);
         dev::tma_load_2d(dev::smem_addr(w + kWBytes), &tm_t, kb * kBlock, t0, bar);
-        if (++s == g.stages) s = 0, ph ^= 1;
       }
-      // left early: the loads in flight land before the CTA ends
-      if (kb < kb1)
-        for (int i = 0; i < g.stages && kb - 1 - i >= kb0; ++i) {
-          const int it = kb - 1 - i - kb0;
-          dev::mbar_wait_bounded(dev::smem_addr(&full[it % g.stages]), (it / g.stages) & 1,
-                                 100000000ull);
-        }
+      __syncwarp();
+      if (++s == g.stages) s = 0, ph ^= 1;
     }
+    // left early: the loads in flight land before the CTA ends
+    if (kb < kb1)
+      for (int i = 0; i < g.stages && kb - 1 - i >= kb0; ++i) {
+        const int it = kb - 1 - i - kb0;
+        dev::mbar_wait_bounded(dev::smem_addr(&full[it % g.stages]), (it / g.stages) & 1,
+                               100000000ull);
+      }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int s = 0, i = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int b = kb0 >> 2; b <= (kb1 - 1) >> 2 && ok; ++b, ++i) {
-        const int slot = i & 1;
-        if (!wait(&sfull[slot], (i >> 1) & 1)) break;
-        tc::fence_after_sync();
-        const uint32_t words = dev::smem_addr(scales + slot * kScaleSlot);
-        const uint32_t sf_w = tmem + kScaleCol + 4 * slot, sf_t = tmem + kScaleCol + 8 + 8 * slot;
+    int s = 0, i = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int b = kb0 >> 2; b <= (kb1 - 1) >> 2 && ok; ++b, ++i) {
+      const int slot = i & 1, piece = (b >> 2) - (kb0 >> 4), buf = piece & 1;
+      if ((i == 0 || (b & 3) == 0) && !wait(&sfull[buf], (piece >> 1) & 1)) break;
+      // the MMAs of the batch before the last have read this slot's scales
+      if (!wait(&bdone[slot], ((i >> 1) & 1) ^ 1)) break;
+      tc::fence_after_sync();
+      const uint32_t words = dev::smem_addr(scales + (4 * buf + (b & 3)) * kSplitSlot);
+      const uint32_t sf_w = tmem + g.n + 4 * slot, sf_t = tmem + g.n + 8 + 4 * slot;
+      if (dev::elect_one()) {
         tc::cp_scales<1>(sf_w, tc::rows16_desc(words));
         tc::cp_scales<1>(sf_t, tc::rows16_desc(words + 512));
-        if (g.n > 128) tc::cp_scales<1>(sf_t + 4, tc::rows16_desc(words + 1024));
-        for (int kb = max(kb0, 4 * b); kb < min(kb1, 4 * b + 4); ++kb) {
-          if (!wait(&full[s], ph)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after_sync();
-          const uint32_t w = dev::smem_addr(ring + (size_t)s * stage_bytes);
-          const uint64_t dw = tc::sw128_kmajor_desc(w), dt = tc::sw128_kmajor_desc(w + kWBytes);
-          const uint32_t idesc = tc::instr_desc_block_scaled(128, g.n, kb & 3);
+      }
+      __syncwarp();
+      const int end = min(kb1, 4 * b + 4);
+      for (int kb = max(kb0, 4 * b); kb < end; ++kb) {
+        if (!wait(&full[s], ph)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        const uint32_t w = dev::smem_addr(ring + (size_t)s * stage_bytes);
+        const uint64_t dw = tc::sw128_kmajor_desc(w), dt = tc::sw128_kmajor_desc(w + kWBytes);
+        const uint32_t idesc = tc::instr_desc_block_scaled(128, g.n, kb & 3);
+        if (dev::elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             tc::mma_block_scaled<1>(tmem, dw + 2 * k, dt + 2 * k, idesc, sf_w, sf_t,
                                     (kb != kb0 || k != 0) ? 1u : 0u);
           tc::commit<1>(dev::smem_addr(&empty[s]));
-          if (++s == g.stages) s = 0, ph ^= 1;
         }
-        tc::commit<1>(dev::smem_addr(&sfree[slot]));
+        __syncwarp();
+        if (++s == g.stages) s = 0, ph ^= 1;
       }
-      tc::commit<1>(dev::smem_addr(&done));
-      // every MMA issued above is complete once `done` flips
-      if (!dev::mbar_wait_bounded(dev::smem_addr(&done), 0))
-        dev::report_status(g.status, CMB_ERR_TIMEOUT);
+      if (dev::elect_one()) {
+        tc::commit<1>(dev::smem_addr(&bdone[slot]));
+        if ((b & 3) == 3) tc::commit<1>(dev::smem_addr(&sfree[buf]));
+      }
+      __syncwarp();
     }
+    if (dev::elect_one()) tc::commit<1>(dev::smem_addr(&done));
+    __syncwarp();
+    // every MMA issued above is complete once `done` flips
+    if (!dev::mbar_wait_bounded(dev::smem_addr(&done), 0))
+      dev::report_status(g.status, CMB_ERR_TIMEOUT);
   } else if (warp == 2) {
     int i = 0;
-    for (int b = kb0 >> 2; b <= (kb1 - 1) >> 2; ++b, ++i) {
-      uint32_t w[4], t[2][4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        w[c] = scale_word(g.scale_w, g.ld_scale_w, w0 + 32 * c + lane, g.w_rows, g.w_shift, b,
-                          g.groups, g.w_words);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = 128 * j + 32 * c + lane;
-          t[j][c] = r < g.n ? scale_word(g.scale_t, g.ld_scale_t, t0 + r, g.t_rows, 0, b, g.groups,
-                                         g.t_words)
-                            : 0u;
-        }
-      }
-      const int slot = i & 1;
-      if (!wait(&sfree[slot], ((i >> 1) & 1) ^ 1)) break;
-      const uint32_t words = dev::smem_addr(scales + slot * kScaleSlot) + 16 * lane;
-      st_shared_v4(words, w);
-      st_shared_v4(words + 512, t[0]);
-      if (g.n > 128) st_shared_v4(words + 1024, t[1]);
+    for (int b = kb0 >> 4; b <= (kb1 - 1) >> 4; ++b, ++i) {
+      uint4 w[4], t[4];
+      scale_pieces<1>(w, g.scale_w, g.ld_scale_w, w0 + lane, g.w_rows, g.w_shift, b, g.groups,
+                      g.w_vec);
+      scale_pieces<1>(t, g.scale_t, g.ld_scale_t, t0 + lane, g.t_rows, 0, b, g.groups, g.t_vec);
+      const int buf = i & 1;
+      if (!wait(&sfree[buf], ((i >> 1) & 1) ^ 1)) break;
+      const uint32_t at = dev::smem_addr(scales + buf * 4 * kSplitSlot) + 16 * lane;
+      put_pieces<1>(at, kSplitSlot, w);
+      put_pieces<1>(at + 512, kSplitSlot, t);
       dev::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) dev::mbar_arrive(dev::smem_addr(&sfull[slot]));
+      if (lane == 0) dev::mbar_arrive(dev::smem_addr(&sfull[buf]));
     }
   } else if (warp >= 4) {
     const bool ok = wait(&done, 0);
@@ -240,28 +363,40 @@ __global__ void __launch_bounds__(256, 1)
       uint32_t r[16];
       tc::ld_32x32b_x16(tmem + (static_cast<uint32_t>(row & 96) << 16) + c0, r);
       tc::wait_ld();
+      if (g.split > 1) {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        if (g.split > 1)
-          mine[(c0 + c) * 128] = __uint_as_float(r[c]);
-        else if (t0 + c0 + c < g.t_rows && w0 + row < g.w_rows)
-          store_c(g, t0 + c0 + c, w0 + row, __uint_as_float(r[c]));
+        for (int c = 0; c < 16; ++c) mine[(c0 + c) * 128] = __uint_as_float(r[c]);
+      } else {
+        store_columns<16>(g, t0 + c0, w0 + row, r);
       }
     }
   }
 
   if (g.split > 1) {
-    // Each CTA finishes 128 / split columns of the tile for every token.
+    // Each CTA finishes 128 / split columns of the tile for every token, four
+    // neighbours a thread, its parts' loads all in flight at once.
     tc::cluster_sync();
-    const int rows = 128 / g.split, first = part * rows;
+    const int quads = 32 / g.split;
     const int tokens = min(g.n, g.t_rows - t0);
-    for (int i = threadIdx.x; i < rows * tokens; i += blockDim.x) {
-      const int row = first + i % rows, t = i / rows;
-      if (w0 + row >= g.w_rows) continue;
+    for (int i = threadIdx.x; i < quads * tokens; i += blockDim.x) {
+      const int row = 4 * (part * quads + i % quads), t = i / quads;
       const uint32_t at = dev::smem_addr(reinterpret_cast<float *>(ring) + t * 128 + row);
-      float v = 0.0f;
-      for (int p = 0; p < g.split; ++p) v += ld_cluster_f32(tc::map_to_cta(at, p));
-      store_c(g, t0 + t, w0 + row, v);
+      float4 v[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        v[p] = p < g.split ? ld_cluster_f4(tc::map_to_cta(at, p)) : make_float4(0, 0, 0, 0);
+      float4 sum = v[0];
+#pragma unroll
+      for (int p = 1; p < 8; ++p) {
+        sum.x += v[p].x;
+        sum.y += v[p].y;
+        sum.z += v[p].z;
+        sum.w += v[p].w;
+      }
+      const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (w0 + row + c < g.w_rows) store_c(g, t0 + t, w0 + row + c, out[c]);
     }
     tc::cluster_sync();  // nobody's shared memory goes while another reads it
   }
@@ -269,48 +404,387 @@ __global__ void __launch_bounds__(256, 1)
   __syncthreads();
   if (warp == 1) {
     tc::fence_after_sync();
-    tc::tmem_dealloc<1>(tmem, 512);
+    tc::tmem_dealloc<1>(tmem, g.tmem_cols);
   }
 }
 
-int launch_split(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
-                 cudaStream_t stream) {
-  // Even shares of the tokens, in steps of 16.
-  const int tiles_t = (g.t_rows + 255) / 256;
-  g.n = ((g.t_rows + tiles_t - 1) / tiles_t + 15) / 16 * 16;
-  const long long tiles = static_cast<long long>((g.w_rows + 127) / 128) *
-                          ((g.t_rows + g.n - 1) / g.n);
-  g.split = 1;
-  while (g.split < 8 && tiles * g.split * 2 <= current_sm_count() && g.groups >= g.split * 2)
-    g.split *= 2;
-  if (tiles * g.split > 0x7fffffffLL) return fail(CMB_ERR_INVALID_ARG, "gemm: too many tiles");
-  const int stage_bytes = kWBytes + g.n * 128;
-  g.stages = static_cast<int>((kSmemMost - 1024 - 2 * kScaleSlot) / stage_bytes);
+// ------------------------------------------------ many tokens: CTA pairs
+
+constexpr int kPairThreads = 384;
+
+__device__ __forceinline__ void tile_at(int t, int tiles_w, int tiles_t, int &tw, int &tt) {
+  // 8 rows of tiles advance together along the tokens, so the pairs at work
+  // at one time share weights and tokens in L2.
+  const int per_group = 8 * tiles_t, first = t / per_group * 8;
+  const int high = min(tiles_w - first, 8), r = t % per_group;
+  tw = first + r % high;
+  tt = r / high;
+}
+
+// A cluster of two CTAs walks over tiles of 256 weight rows x n token rows (n
+// a multiple of 32, up to 256): cta_group::2 MMAs issued by CTA 0, each CTA
+// loading its 128 weight rows and half of the token rows.  Up to n = 224 TMEM
+// holds two accumulators beside the scales, so a tile's MMAs run while the
+// last one is stored.
+//   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-11 accumulators
+__global__ void __launch_bounds__(kPairThreads, 1)
+    k_gemm_pair(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t,
+                const Args g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
+  __shared__ __align__(8) uint64_t sfull[2], sfree[2], bdone[2], tfull[2], tempty[2], done;
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_flag;
+
+  const int n = g.n, bufs = 2 * n <= kScaleCol ? 2 : 1;  // accumulators
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = uniform(tc::cluster_ctarank());
+  const int stage_bytes = kWBytes + n / 2 * 128;
+  uint8_t *scales = ring + (size_t)g.stages * stage_bytes;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      dev::mbar_init(dev::smem_addr(&full[s]), 1);
+      dev::mbar_init(dev::smem_addr(&empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      dev::mbar_init(dev::smem_addr(&sfull[s]), 2);  // both CTAs' words
+      dev::mbar_init(dev::smem_addr(&sfree[s]), 1);
+      dev::mbar_init(dev::smem_addr(&bdone[s]), 1);
+      dev::mbar_init(dev::smem_addr(&tfull[s]), 1);
+      dev::mbar_init(dev::smem_addr(&tempty[s]), 16);  // 8 warps of both CTAs
+    }
+    dev::mbar_init(dev::smem_addr(&done), 1);
+    abort_flag = 0;
+    dev::fence_mbar_init();
+    dev::tma_prefetch_desc(&tm_w);
+    dev::tma_prefetch_desc(&tm_t);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc<2>(dev::smem_addr(&tmem_holder), 512);
+    tc::tmem_relinquish<2>();
+  }
+  tc::fence_before_sync();
+  tc::cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = uniform(tmem_holder);
+  const int tiles_w = (g.w_rows + 255) / 256, tiles_t = (g.t_rows + n - 1) / n;
+  const int tiles = tiles_w * tiles_t, first = blockIdx.x / 2, step = gridDim.x / 2;
+  const Waiter wait{&abort_flag, g.status};
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
+
+  // Warps 0 and 1 stay whole and elect a lane for each issue: their operands
+  // are then warp-uniform, which the tensor core's and TMA's instructions need.
+  if (warp == 0) {
+    int s = 0, armed = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      int tw, tt;
+      tile_at(t, tiles_w, tiles_t, tw, tt);
+      const int w_row = tw * 256 + rank * 128, t_row = tt * n + rank * (n / 2);
+      for (int kb = 0; kb < g.groups; ++kb) {
+        if (!wait(&empty[s], ph ^ 1)) {
+          ok = false;
+          break;
+        }
+        uint8_t *w = ring + (size_t)s * stage_bytes;
+        // both CTAs' loads complete on CTA 0's barrier
+        const uint32_t bar = tc::map_to_cta(dev::smem_addr(&full[s]), 0);
+        if (dev::elect_one()) {
+          if (rank == 0) dev::mbar_arrive_expect_tx(dev::smem_addr(&full[s]), 2 * stage_bytes);
+          tc::tma_load_2d_pair(dev::smem_addr(w), &tm_w, kb * kBlock, w_row, bar);
+          tc::tma_load_2d_pair(dev::smem_addr(w + kWBytes), &tm_t, kb * kBlock, t_row, bar);
+        }
+        __syncwarp();
+        ++armed;
+        if (++s == g.stages) s = 0, ph ^= 1;
+      }
+    }
+    // left early: the loads in flight land before the pair ends
+    if (!ok && rank == 0)
+      for (int i = 0; i < g.stages && armed - 1 - i >= 0; ++i) {
+        const int it = armed - 1 - i;
+        dev::mbar_wait_bounded(dev::smem_addr(&full[it % g.stages]), (it / g.stages) & 1,
+                               100000000ull);
+      }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      int s = 0, j = 0;
+      uint32_t ph = 0;
+      unsigned i = 0, piece = 0;  // batches of four K blocks and of sixteen, over all tiles
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step, ++j) {
+        const int a = j % bufs;
+        if (!wait.of_pair(&tempty[a], (static_cast<uint32_t>(j / bufs) & 1) ^ 1)) break;
+        const uint32_t d = tmem + a * n;
+        for (int b = 0; 4 * b < g.groups && ok; ++b, ++i) {
+          const int slot = i & 1, buf = piece & 1, kend = min(g.groups, 4 * b + 4);
+          // the MMAs of the batch before the last have read this slot's scales
+          if (((b & 3) == 0 && !wait.of_pair(&sfull[buf], (piece >> 1) & 1)) ||
+              !wait(&bdone[slot], ((i >> 1) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+          const uint32_t words = dev::smem_addr(scales + (4 * buf + (b & 3)) * kScaleSlot);
+          const uint32_t sf_w = tmem + kScaleCol + 4 * slot, sf_t = tmem + kScaleCol + 8 + 8 * slot;
+          if (dev::elect_one()) {
+            tc::cp_scales<2>(sf_w, tc::rows16_desc(words));
+            tc::cp_scales<2>(sf_t, tc::rows16_desc(words + 512));
+            if (n > 128) tc::cp_scales<2>(sf_t + 4, tc::rows16_desc(words + 1024));
+          }
+          __syncwarp();
+          for (int kb = 4 * b; kb < kend; ++kb) {
+            if (!wait(&full[s], ph)) {
+              ok = false;
+              break;
+            }
+            tc::fence_after_sync();
+            const uint32_t w = dev::smem_addr(ring + (size_t)s * stage_bytes);
+            const uint64_t dw = tc::sw128_kmajor_desc(w), dt = tc::sw128_kmajor_desc(w + kWBytes);
+            const uint32_t idesc = tc::instr_desc_block_scaled(256, n, kb & 3);
+            if (dev::elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc::mma_block_scaled<2>(d, dw + 2 * k, dt + 2 * k, idesc, sf_w, sf_t,
+                                        (kb | k) != 0 ? 1u : 0u);
+              tc::commit_pair(dev::smem_addr(&empty[s]));
+            }
+            __syncwarp();
+            if (++s == g.stages) s = 0, ph ^= 1;
+          }
+          const bool last = (b & 3) == 3 || kend == g.groups;  // of its 16 K blocks
+          if (dev::elect_one()) {
+            tc::commit<2>(dev::smem_addr(&bdone[slot]));
+            if (last) tc::commit_pair(dev::smem_addr(&sfree[buf]));
+          }
+          __syncwarp();
+          if (last) ++piece;
+        }
+        if (!ok) break;
+        if (dev::elect_one()) tc::commit_pair(dev::smem_addr(&tfull[a]));
+        __syncwarp();
+      }
+      // every MMA issued above is complete once `done` flips
+      if (dev::elect_one()) tc::commit<2>(dev::smem_addr(&done));
+      __syncwarp();
+      if (!dev::mbar_wait_bounded(dev::smem_addr(&done), 0))
+        dev::report_status(g.status, CMB_ERR_TIMEOUT);
+    }
+  } else if (warp == 2) {
+    unsigned i = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      int tw, tt;
+      tile_at(t, tiles_w, tiles_t, tw, tt);
+      for (int b = 0; 16 * b < g.groups; ++b, ++i) {
+        uint4 w[4], tv[8];
+        scale_pieces<1>(w, g.scale_w, g.ld_scale_w, tw * 256 + rank * 128 + lane, g.w_rows,
+                        g.w_shift, b, g.groups, g.w_vec);
+        scale_pieces<2>(tv, g.scale_t, g.ld_scale_t, tt * n + lane, g.t_rows, 0, b, g.groups,
+                        g.t_vec);
+        const int buf = i & 1;
+        ok = wait(&sfree[buf], ((i >> 1) & 1) ^ 1);
+        if (!ok) break;
+        const uint32_t at = dev::smem_addr(scales + buf * 4 * kScaleSlot) + 16 * lane;
+        put_pieces<1>(at, kScaleSlot, w);
+        put_pieces<2>(at + 512, kScaleSlot, tv);
+        dev::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) dev::mbar_arrive_cluster(tc::map_to_cta(dev::smem_addr(&sfull[buf]), 0));
+      }
+    }
+  } else if (warp >= 4) {
+    const int q = warp & 3, h = (warp - 4) >> 2, chunks = n / 16;
+    int j = 0;
+    for (int t = first; t < tiles; t += step, ++j) {
+      int tw, tt;
+      tile_at(t, tiles_w, tiles_t, tw, tt);
+      const int a = j % bufs;
+      if (!wait(&tfull[a], static_cast<uint32_t>(j / bufs) & 1)) break;
+      tc::fence_after_sync();
+      const int w = tw * 256 + rank * 128 + q * 32 + lane;
+      const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + a * n;
+      for (int c = h; c < chunks; c += 2) {
+        uint32_t r[16];
+        tc::ld_32x32b_x16(at + 16 * c, r);
+        tc::wait_ld();
+        if (c + 2 >= chunks) {  // read to the end: hand it back, then store
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) dev::mbar_arrive_cluster(tc::map_to_cta(dev::smem_addr(&tempty[a]), 0));
+        }
+        store_columns<16>(g, tt * n + 16 * c, w, r);
+      }
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc<2>(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------- launches
+
+int launch_kernel(void (*kernel)(CUtensorMap, CUtensorMap, Args), const uint8_t *A, size_t lda,
+                const uint8_t *B, size_t ldb, Args g, int t_box, long long ctas, int cluster,
+                int threads, int slot_bytes, size_t smem_most, cudaStream_t stream) {
+  const int stage_bytes = kWBytes + t_box * 128;
+  g.stages = static_cast<int>((smem_most - 1024 - 8 * slot_bytes) / stage_bytes);
   if (g.stages > kMaxStages) g.stages = kMaxStages;
-  const size_t smem = (size_t)g.stages * stage_bytes + 2 * kScaleSlot + 1024;
+  if (ctas > 0x7fffffffLL) return fail(CMB_ERR_INVALID_ARG, "gemm: too many tiles");
   CUtensorMap tw, tt;
   int rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, g.w_rows, g.K, ldb, 128, kBlock,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (rc) return rc;
-  rc = make_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, g.t_rows, g.K, lda, g.n, kBlock,
+  rc = make_tmap_2d(&tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, g.t_rows, g.K, lda, t_box, kBlock,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
   if (rc) return rc;
-  CMB_CUDA_TRY(cudaFuncSetAttribute(k_gemm_split, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  CMB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(kSmemMost)));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * g.split));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (size_t)g.stages * stage_bytes + 8 * slot_bytes + 1024;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = g.split;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  // the prologue may run while the stream's last kernel ends
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  CMB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm_split, tw, tt, g));
+  cfg.numAttrs = 2;
+  CMB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tw, tt, g));
   return CMB_OK;
+}
+
+// Clusters of 1, 2, 4 and 8 CTAs of k_gemm_split that the device holds at one
+// a SM (148, 74, 33 and 15 on a B200: clusters stay within a GPC).
+struct ClusterRoom {
+  int clusters[4];
+};
+
+ClusterRoom cluster_room() {
+  constexpr int kMaxDevices = 64;
+  static std::mutex mu;
+  static ClusterRoom known[kMaxDevices];
+  const int sms = current_sm_count();
+  ClusterRoom room = {{sms, sms / 2, sms / 5, sms / 11}};  // where the query fails
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return room;
+  std::lock_guard<std::mutex> lock(mu);
+  if (known[device].clusters[0] != 0) return known[device];
+  cudaFuncSetAttribute(k_gemm_split, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       static_cast<int>(kSmemMost));
+  for (int i = 0; i < 4; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << i);
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = kSmemMost;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << i;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, k_gemm_split, &cfg) == cudaSuccess && n > 0)
+      room.clusters[i] = n;
+  }
+  return known[device] = room;
+}
+
+// How a product is cut: `n` tokens a tile, the K of a tile over `split` CTAs
+// (0: k_gemm_pair), and whether two CTAs share a SM.
+struct Cut {
+  int n, split;
+  bool two;
+};
+
+long long tiles_of(const Args &g, int w, int n) {
+  return static_cast<long long>((g.w_rows + w - 1) / w) * ((g.t_rows + n - 1) / n);
+}
+
+// The cut that takes least time by a model of both kernels in microseconds,
+// fitted to 9000 timings (18 weight shapes from 128 x 8192 to 16384 x 2048,
+// 1-8192 tokens, every cut): it picks one within 2 % of the fastest on
+// average.  A K block takes a CTA ~0.27 us however few its tokens; a SM that
+// two CTAs share, or a pair, is bound by the bytes that reach it (~0.13 us +
+// 0.5 ns a token; 0.21 us + 0.5 ns); all of it by reading the operands once
+// (5.7 GB/ms).  What a cut adds: parts to sum (0.27 us a doubling + 20 ns a
+// token), columns to store, a wave that starts over.  Some of what it weighs
+// (us): 1 x 8192 x 8192 split 1/2/4: 19.5/14.3/13.7, pairs 20.4; 256 x 8192 x
+// 8192 split 1 at n 128: 21.4, pairs 22.4; 1000 x 4600 x 2064 split 16.9, pairs
+// at n 128/224/256: 17.3/20.3/13.3.
+Cut choose_cut(const Args &g) {
+  const ClusterRoom room = cluster_room();
+  const double read = (static_cast<double>(g.w_rows) + g.t_rows) * g.K / 1e6;
+  Cut best = {256, 0, false};
+  double least = 1e30;
+  for (int n = 32; n <= 256; n += 32) {
+    const long long waves = (tiles_of(g, 256, n) + current_sm_count() / 2 - 1) /
+                            (current_sm_count() / 2);
+    const double us = 4.05 + fmax(waves * g.groups * (0.208 + 0.00047 * n), 0.185 * read) +
+                      0.0087 * n + (2 * n > kScaleCol ? 3.0 * (waves - 1) : 0.0);
+    if (us < least) least = us, best = {n, 0, false};
+    if (n >= g.t_rows) break;
+  }
+  // even shares of the tokens in steps of 16, up to 128 a tile
+  const int fewest = (g.t_rows + 127) / 128;
+  int last = 0;
+  for (int parts = fewest; parts < fewest + 8; ++parts) {
+    const int n = ((g.t_rows + parts - 1) / parts + 15) / 16 * 16;
+    if (n == last || (parts > 1 && n < 48)) continue;
+    last = n;
+    const long long tiles = tiles_of(g, 128, n);
+    for (int i = 0; i < 4 && g.groups >= 1 << i; ++i) {
+      const long long load = (tiles + room.clusters[i] - 1) / room.clusters[i];
+      // k_gemm_split takes one tile a cluster: past two waves pairs, which
+      // persist, are ahead, but for the single row of tiles of a wide layer
+      if (load > 2 && (i > 0 || g.t_rows > n)) continue;
+      const int blocks = (g.groups + (1 << i) - 1) >> i;
+      double each = load * (0.133 + 0.0005 * n);
+      if (load == 1) each = fmax(each, 0.267);
+      const double us = 2.1 + fmax(blocks * each, 0.176 * read) + 0.0103 * n * load -
+                        0.33 * (load - 1) + (i > 0 ? 0.27 * i + 0.0196 * n * load : 0.0);
+      // one CTA a SM where each has a place of its own and tiles are large:
+      // twice the stages (128 x 8192 x 8192 by halves: 18.2 us against 21.1);
+      // else two, and the next kernel's may start beside it (1 x 4096 x 4096
+      // by quarters: 5.5 against 6.2)
+      if (us < least) least = us, best = {n, 1 << i, load > 1 || n <= 48};
+    }
+  }
+  return best;
+}
+
+int launch(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
+           cudaStream_t stream) {
+  const Cut cut = choose_cut(g);
+  g.n = cut.n;
+  if (cut.split == 0) {
+    const long long tiles = tiles_of(g, 256, g.n);
+    if (tiles > 0x3fffffffLL) return fail(CMB_ERR_INVALID_ARG, "gemm: too many tiles");
+    const int pairs = current_sm_count() / 2;
+    return launch_kernel(k_gemm_pair, A, lda, B, ldb, g, g.n / 2, 2 * (tiles < pairs ? tiles : pairs),
+                         2, kPairThreads, kScaleSlot, kSmemMost, stream);
+  }
+  g.split = cut.split;
+  g.tmem_cols = 32;
+  while (g.tmem_cols < g.n + 16) g.tmem_cols *= 2;
+  return launch_kernel(k_gemm_split, A, lda, B, ldb, g, g.n, tiles_of(g, 128, g.n) * g.split,
+                       g.split, kSplitThreads, kSplitSlot, cut.two ? kSmemHalf : kSmemMost, stream);
 }
 
 }  // namespace
@@ -363,9 +837,9 @@ extern "C" int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_
   g.K = K;
   g.groups = static_cast<int>(groups);
   g.w_shift = block_rows_b == 1 ? 0 : 7;
-  g.w_words = b128::aligned_to(scale_b, ld_scale_b, 4);
-  g.t_words = b128::aligned_to(scale_a, ld_scale_a, 4);
+  g.w_vec = b128::aligned_to(scale_b, ld_scale_b, 16);
+  g.t_vec = b128::aligned_to(scale_a, ld_scale_a, 16);
   g.bf16 = c_type == CMB_BF16;
   g.status = status;
-  return launch_split(A, lda, B, ldb, g, stream);
+  return launch(A, lda, B, ldb, g, stream);
 }

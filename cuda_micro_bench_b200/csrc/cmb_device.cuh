@@ -282,6 +282,20 @@ __device__ __forceinline__ uint64_t policy_evict_last() {
   return p;
 }
 
+// ---------------------------------------------- programmatic launches
+
+// Waits until the grids this one depends on have completed and their writes
+// are visible; nothing to wait for where the launch was an ordinary one.
+__device__ __forceinline__ void grid_dep_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Lets the next grid's launch begin (its own grid_dep_wait still holds it
+// until this grid has completed).
+__device__ __forceinline__ void grid_dep_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ------------------------------------------------------------ warp utils
 
 __device__ __forceinline__ bool elect_one() {

@@ -2,7 +2,7 @@
 // TMEM allocation, shared-memory matrix descriptors, instruction
 // descriptors, tcgen05.mma / commit / ld, and the cluster helpers the
 // 2-CTA (cta_group::2) GEMM needs.  Nothing here addresses another GPU's
-// memory, and no load or commit names more than one destination CTA.
+// memory, and no load names more than one destination CTA.
 #pragma once
 
 #include <cstdint>
@@ -200,6 +200,16 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::
                      "r"(bar)
                  : "memory");
+}
+
+// The same arrival on the mbarriers at that place of both CTAs of a pair
+// (`bar`: the shared::cta address), by one instruction.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
 }
 
 // ------------------------------------------------------------ TMEM -> regs
