@@ -43,22 +43,51 @@ __device__ __forceinline__ float scale_reciprocal(uint32_t byte) {
   return __uint_as_float((254u - byte) << 23);
 }
 
+// Magnitudes compare like their bits, so a maximum is an integer one, and one
+// look at it tells whether a block has anything that is not finite.
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+__device__ __forceinline__ uint32_t magnitude_bits(float x) {
+  return __float_as_uint(x) & 0x7FFFFFFFu;
+}
+
 // Two values to e4m3 (nearest even), `lo` in the low byte.  The scale keeps
-// finite values within 448, so saturation only ever meets infinities; those
-// become NaN, as NaN does.
+// finite values within 448, so saturation only ever meets infinities; where a
+// block may hold any (kAny), those become NaN, as NaN does.
+template <bool kAny>
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint32_t v = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-  if (!(fabsf(lo) <= kMaxFinite)) v = (v & 0xFF00u) | 0x7Fu;
-  if (!(fabsf(hi) <= kMaxFinite)) v = (v & 0x00FFu) | 0x7F00u;
+  if constexpr (kAny) {
+    if (!(fabsf(lo) <= kMaxFinite)) v = (v & 0xFF00u) | 0x7Fu;
+    if (!(fabsf(hi) <= kMaxFinite)) v = (v & 0x00FFu) | 0x7F00u;
+  }
   return v;
 }
 
+// a * s, both halves at once.
+__device__ __forceinline__ float2 mul2(float2 a, float2 s) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(s.x), "f"(s.y));
+  return r;
+}
+
 // 8 values times `inv` as 8 e4m3 bytes.
+template <bool kAny>
 __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
-  uint2 q;
-  q.x = e4m3x2(v[0] * inv, v[1] * inv) | (e4m3x2(v[2] * inv, v[3] * inv) << 16);
-  q.y = e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16);
-  return q;
+  const float2 s = make_float2(inv, inv);
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = mul2(make_float2(v[2 * i], v[2 * i + 1]), s);
+    h[i] = e4m3x2<kAny>(p.x, p.y);
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
 // ------------------------------------------------- rows of bf16 or fp32
@@ -112,6 +141,19 @@ __device__ __forceinline__ void unpack(const Raw8<float> &r, float (&v)[8]) {
   const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+}
+
+// Largest magnitude's bits (as fp32 bits) of the 8; NaN and infinities count.
+__device__ __forceinline__ uint32_t top_bits(const Raw8<__nv_bfloat16> &r) {
+  const uint32_t m = 0x7FFF7FFFu;
+  const uint32_t v =
+      __vmaxu2(__vmaxu2(r.a.x & m, r.a.y & m), __vmaxu2(r.a.z & m, r.a.w & m));
+  return max(v << 16, v & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t top_bits(const Raw8<float> &r) {
+  const uint32_t m = 0x7FFFFFFFu;
+  return max(max(max(r.a.x & m, r.a.y & m), max(r.a.z & m, r.a.w & m)),
+             max(max(r.b.x & m, r.b.y & m), max(r.b.z & m, r.b.w & m)));
 }
 
 __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {

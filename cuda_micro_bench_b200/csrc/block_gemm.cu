@@ -722,13 +722,14 @@ long long tiles_of(const Args &g, int w, int n) {
 // 1-8192 tokens, every cut): it picks one within 2 % of the fastest on
 // average.  A K block takes a CTA ~0.27 us however few its tokens; a SM that
 // two CTAs share, or a pair, is bound by the bytes that reach it (~0.13 us +
-// 0.5 ns a token; 0.21 us + 0.5 ns); all of it by reading the operands once
-// (5.7 GB/ms).  What a cut adds: parts to sum (0.27 us a doubling + 20 ns a
+// 0.7 ns a token; 0.21 us + 0.5 ns; more where rows do not start on 128 bytes,
+// `skewed`, and each 128 bytes of a row lie in two lines); all of it by
+// reading the operands once (5.6 GB/ms).  What a cut adds: parts to sum (0.28 us a doubling + 20 ns a
 // token), columns to store, a wave that starts over.  Some of what it weighs
 // (us): 1 x 8192 x 8192 split 1/2/4: 19.5/14.3/13.7, pairs 20.4; 256 x 8192 x
 // 8192 split 1 at n 128: 21.4, pairs 22.4; 1000 x 4600 x 2064 split 16.9, pairs
 // at n 128/224/256: 17.3/20.3/13.3.
-Cut choose_cut(const Args &g) {
+Cut choose_cut(const Args &g, bool skewed) {
   const ClusterRoom room = cluster_room();
   const double read = (static_cast<double>(g.w_rows) + g.t_rows) * g.K / 1e6;
   Cut best = {256, 0, false};
@@ -736,8 +737,9 @@ Cut choose_cut(const Args &g) {
   for (int n = 32; n <= 256; n += 32) {
     const long long waves = (tiles_of(g, 256, n) + current_sm_count() / 2 - 1) /
                             (current_sm_count() / 2);
-    const double us = 4.05 + fmax(waves * g.groups * (0.208 + 0.00047 * n), 0.185 * read) +
-                      0.0087 * n + (2 * n > kScaleCol ? 3.0 * (waves - 1) : 0.0);
+    const double us = 3.93 + fmax(waves * g.groups * (0.205 + 0.0005 * n) * (skewed ? 1.26 : 1.0),
+                                  0.194 * read) +
+                      0.007 * n + (2 * n > kScaleCol ? 3.0 * (waves - 1) : 0.0);
     if (us < least) least = us, best = {n, 0, false};
     if (n >= g.t_rows) break;
   }
@@ -755,10 +757,10 @@ Cut choose_cut(const Args &g) {
       // persist, are ahead, but for the single row of tiles of a wide layer
       if (load > 2 && (i > 0 || g.t_rows > n)) continue;
       const int blocks = (g.groups + (1 << i) - 1) >> i;
-      double each = load * (0.133 + 0.0005 * n);
-      if (load == 1) each = fmax(each, 0.267);
-      const double us = 2.1 + fmax(blocks * each, 0.176 * read) + 0.0103 * n * load -
-                        0.33 * (load - 1) + (i > 0 ? 0.27 * i + 0.0196 * n * load : 0.0);
+      double each = load * (0.134 + 0.0007 * n) * (skewed ? 1.7 : 1.0);
+      if (load == 1) each = fmax(each, 0.266);
+      const double us = 2.14 + fmax(blocks * each, 0.178 * read) + 0.0086 * n * load -
+                        0.55 * (load - 1) + (i > 0 ? 0.28 * i + 0.02 * n * load : 0.0);
       // one CTA a SM where each has a place of its own and tiles are large:
       // twice the stages (128 x 8192 x 8192 by halves: 18.2 us against 21.1);
       // else two, and the next kernel's may start beside it (1 x 4096 x 4096
@@ -771,7 +773,7 @@ Cut choose_cut(const Args &g) {
 
 int launch(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
            cudaStream_t stream) {
-  const Cut cut = choose_cut(g);
+  const Cut cut = choose_cut(g, lda % 128 != 0 || ldb % 128 != 0);
   g.n = cut.n;
   if (cut.split == 0) {
     const long long tiles = tiles_of(g, 256, g.n);

@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) k_quantize_tile(const QuantArgs a) {
         b128::unpack(raw[i], v);
         if (ncol > 0)
           b128::store_bytes(a.dst + (size_t)(row + i) * a.ld_dst + col,
-                            b128::e4m3x8(v, b128::scale_reciprocal(rbyte[i])), ncol, a.dst_vec);
+                            b128::e4m3x8<true>(v, b128::scale_reciprocal(rbyte[i])), ncol, a.dst_vec);
         if (a.block_rows == 1 && col_in == 0)
           a.scale[(size_t)(row + i) * a.ld_scale + blockIdx.x] = static_cast<uint8_t>(rbyte[i]);
       }
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) k_quantize_tile(const QuantArgs a) {
         }
         if (nrow > 0)
           b128::store_bytes(a.dst_t + (size_t)(col + j) * a.ld_dst_t + row,
-                            b128::e4m3x8(v, b128::scale_reciprocal(cbyte[j])), nrow, a.dst_t_vec);
+                            b128::e4m3x8<true>(v, b128::scale_reciprocal(cbyte[j])), nrow, a.dst_t_vec);
         if (a.block_rows == 1 && row_in == 0)
           a.scale_t[(size_t)(col + j) * a.ld_scale_t + tile_r] = static_cast<uint8_t>(cbyte[j]);
       }

@@ -7,6 +7,13 @@
 // Memory bound.  h is rounded to the rows' type before the mean: the norm,
 // its backward pass and every later reader then see the same h.  Sums and
 // statistics are fp32, in a fixed order.
+//
+// A CTA works on a whole row.  Two ways to read rows (template kRing):
+//   ring    rows that start and end on 16 bytes, several rows a CTA: a thread
+//           keeps the next rows on their way into shared memory with bulk
+//           copies, so loads never wait for a row's reduction.
+//   direct  everything else, and calls with no more rows than CTAs, whose
+//           latency is one load.
 #include "block128.cuh"
 #include "cmb_host.h"
 
@@ -16,6 +23,7 @@ namespace {
 using b128::Raw8;
 
 constexpr int kMaxParts = 1024;  // rows of partial weight gradients in the workspace
+constexpr int kStages = 3;       // rows in the ring
 
 // Sum over the CTA, the same value in every thread.  `part` holds one float
 // for each warp; two calls in a row use different ones.
@@ -32,6 +40,46 @@ __device__ __forceinline__ float cta_sum(float v, float *part) {
   return v;
 }
 
+// Rows of up to three matrices on their way through shared memory: row i of
+// a CTA (its rows are blockIdx.x, + gridDim.x, ...) in stage i % kStages.
+struct Ring {
+  const uint8_t *src[3];
+  size_t pitch[3];
+  int n;          // matrices
+  uint32_t bytes;  // of a row of one of them
+  uint8_t *mem;
+  uint64_t *full;
+
+  __device__ __forceinline__ void load(int i, int rows) const {
+    const long long row = blockIdx.x + static_cast<long long>(i) * gridDim.x;
+    if (row >= rows) return;
+    const int s = i % kStages;
+    const uint32_t bar = dev::smem_addr(full + s);
+    dev::mbar_arrive_expect_tx(bar, bytes * n);
+    for (int k = 0; k < n; ++k)
+      dev::bulk_load(dev::smem_addr(mem + (size_t)(s * n + k) * bytes), src[k] + row * pitch[k],
+                     bytes, bar);
+  }
+  __device__ __forceinline__ void start(int rows) const {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < kStages; ++s) dev::mbar_init(dev::smem_addr(full + s), 1);
+      dev::fence_mbar_init();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int s = 0; s < kStages; ++s) load(s, rows);
+  }
+  // Waits for row i; a bulk copy of this GPU's own memory ends, or the launch
+  // has failed as a whole.
+  __device__ __forceinline__ void wait(int i) const {
+    dev::mbar_wait_bounded(dev::smem_addr(full + i % kStages), (i / kStages) & 1);
+  }
+  template <typename T>
+  __device__ __forceinline__ const T *row(int i, int k) const {
+    return reinterpret_cast<const T *>(mem + (size_t)(i % kStages * n + k) * bytes);
+  }
+};
+
 struct NormArgs {
   const void *x, *residual, *weight;
   void *h, *y;
@@ -43,70 +91,139 @@ struct NormArgs {
   bool x_vec, r_vec, w_vec, h_vec, y_vec, q_vec;
 };
 
-// One CTA walks over rows; thread t holds the chunks of 8 columns t, t +
-// blockDim, ...: 16 neighbouring threads hold a block of 128.
-template <typename T, typename W, int NV>
-__global__ void __launch_bounds__(1024) k_rmsnorm(const NormArgs a) {
+// The e4m3 values and scales of 8 columns of a row; 16 neighbouring threads
+// have a block of 128.
+__device__ __forceinline__ void store_quantized(const NormArgs &a, int row, int col,
+                                                const float (&y)[8]) {
+  const int n = a.cols - col;
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, b128::magnitude_bits(y[j]));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool any = __any_sync(0xffffffffu, top >= b128::kInfBits);
+  if (any) {  // the scale is that of the finite values
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, b128::finite_magnitude(y[j]));
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    top = __float_as_uint(m);
+  }
+  const uint32_t byte = b128::scale_byte(__uint_as_float(top));
+  const float inv = b128::scale_reciprocal(byte);
+  if (n > 0) {
+    b128::store_bytes(a.q + (size_t)row * a.ld_q + col,
+                      any ? b128::e4m3x8<true>(y, inv) : b128::e4m3x8<false>(y, inv), n, a.q_vec);
+    if ((threadIdx.x & 15) == 0)
+      a.scale[(size_t)row * a.ld_scale + col / b128::kBlock] = static_cast<uint8_t>(byte);
+  }
+}
+
+// A thread's chunks of the weights: kept in registers, or, where a row has
+// more than two chunks a thread, read again for each row.
+template <typename W, int NV>
+struct Weight {
+  const W *p;
+  bool vec;
+  Raw8<W> kept[NV <= 2 ? NV : 1];
+
+  __device__ __forceinline__ Weight(const void *weight, bool aligned, int cols)
+      : p(static_cast<const W *>(weight)), vec(aligned) {
+    if constexpr (NV <= 2) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * blockDim.x + threadIdx.x) * 8;
+        kept[i] = load(col, cols - col);
+      }
+    }
+  }
+  __device__ __forceinline__ Raw8<W> load(int col, int n) const {
+    return n > 0 ? b128::load8_edge(p + col, n, vec) : Raw8<W>{};
+  }
+  __device__ __forceinline__ Raw8<W> chunk(int i, int col, int n) const {
+    if constexpr (NV <= 2) return kept[i];
+    else return load(col, n);
+  }
+};
+
+// Thread t holds the chunks of 8 columns t, t + blockDim, ...: 16
+// neighbouring threads hold a block of 128.
+template <typename T, typename W, int NV, bool kRing>
+__global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
   __shared__ float part[2][32];
+  __shared__ __align__(8) uint64_t full[kStages];
+  extern __shared__ __align__(16) uint8_t rows_mem[];
   const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.residual);
-  const W *w = static_cast<const W *>(a.weight);
-  int turn = 0;
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    float h[NV][8];
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
+  Ring ring;
+  if constexpr (kRing) {
+    ring = {{static_cast<const uint8_t *>(a.x), static_cast<const uint8_t *>(a.residual), nullptr},
+            {a.ld_x * sizeof(T), a.ld_r * sizeof(T), 0},
+            res != nullptr ? 2 : 1,
+            static_cast<uint32_t>(a.cols * sizeof(T)),
+            rows_mem,
+            full};
+    ring.start(a.rows);
+  }
+  const Weight<W, NV> weight(a.weight, a.w_vec, a.cols);
+  int it = 0;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
+    Raw8<T> h[NV];  // as it is stored
     float sq = 0.0f;
+    if constexpr (kRing) ring.wait(it);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      Raw8<T> raw{};
+      Raw8<T> raw{}, add{};
       if (n > 0) {
-        raw = b128::load8_edge(x + (size_t)row * a.ld_x + col, n, a.x_vec);
+        if constexpr (kRing) {
+          raw = b128::load8(ring.row<T>(it, 0) + col);
+          if (res != nullptr) add = b128::load8(ring.row<T>(it, 1) + col);
+        } else {
+          raw = b128::load8_edge(x + (size_t)row * a.ld_x + col, n, a.x_vec);
+          if (res != nullptr) add = b128::load8_edge(res + (size_t)row * a.ld_r + col, n, a.r_vec);
+        }
         if (res != nullptr) {
           float v[8], u[8];
           b128::unpack(raw, v);
-          b128::unpack(b128::load8_edge(res + (size_t)row * a.ld_r + col, n, a.r_vec), u);
+          b128::unpack(add, u);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] += u[j];
           b128::pack(v, raw);
           b128::store8_edge(static_cast<T *>(a.h) + (size_t)row * a.ld_h + col, raw, n, a.h_vec);
         }
       }
-      b128::unpack(raw, h[i]);
+      h[i] = raw;
+      float v[8];
+      b128::unpack(raw, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sq = fmaf(h[i][j], h[i][j], sq);
+      for (int j = 0; j < 8; ++j) sq = fmaf(v[j], v[j], sq);
     }
-    sq = cta_sum(sq, part[turn]);
+    sq = cta_sum(sq, part[it & 1]);
+    if constexpr (kRing)
+      if (threadIdx.x == 0) ring.load(it + kStages, a.rows);  // every thread has its chunks
     const float rstd = 1.0f / sqrtf(sq / static_cast<float>(a.cols) + a.eps);
     if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      float wv[8], top = 0.0f;
-      Raw8<W> wr{};
-      if (n > 0) wr = b128::load8_edge(w + col, n, a.w_vec);
-      b128::unpack(wr, wv);
+      float y[8], wv[8];
+      b128::unpack(h[i], y);
+      b128::unpack(weight.chunk(i, col, n), wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        h[i][j] = h[i][j] * rstd * wv[j];
+        y[j] = y[j] * rstd * wv[j];
         // behind the row's end: not 0 * inf, which would be NaN
-        if (j >= n) h[i][j] = 0.0f;
-        top = fmaxf(top, b128::finite_magnitude(h[i][j]));
+        if (j >= n) y[j] = 0.0f;
       }
       if (a.y != nullptr && n > 0) {
         Raw8<T> out;
-        b128::pack(h[i], out);
+        b128::pack(y, out);
         b128::store8_edge(static_cast<T *>(a.y) + (size_t)row * a.ld_y + col, out, n, a.y_vec);
       }
-      if (a.q != nullptr) {
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t byte = b128::scale_byte(top);
-        if (n > 0) {
-          b128::store_bytes(a.q + (size_t)row * a.ld_q + col,
-                            b128::e4m3x8(h[i], b128::scale_reciprocal(byte)), n, a.q_vec);
-          if ((threadIdx.x & 15) == 0)
-            a.scale[(size_t)row * a.ld_scale + col / b128::kBlock] = static_cast<uint8_t>(byte);
-        }
-      }
+      if (a.q != nullptr) store_quantized(a, row, col, y);
     }
   }
 }
@@ -121,52 +238,72 @@ struct NormBackArgs {
   bool dy_vec, h_vec, dh_vec, w_vec, dx_vec;
 };
 
-template <typename T, typename W, int NV>
-__global__ void __launch_bounds__(1024) k_rmsnorm_back(const NormBackArgs a) {
+// Both passes over a row read it from where it lies, the ring's shared memory
+// or (direct) global memory, so a thread holds no more of it than a chunk; the
+// weight gradient of its columns stays in registers from row to row.
+template <typename T, typename W, int NV, bool kRing>
+__global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) {
   __shared__ float part[2][32];
-  const T *dy = static_cast<const T *>(a.dy), *h = static_cast<const T *>(a.h);
-  const T *dh = static_cast<const T *>(a.dh);
-  const W *w = static_cast<const W *>(a.weight);
+  __shared__ __align__(8) uint64_t full[kStages];
+  extern __shared__ __align__(16) uint8_t rows_mem[];
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
+  Ring ring;
+  if constexpr (kRing) {
+    ring = {{static_cast<const uint8_t *>(a.dy), static_cast<const uint8_t *>(a.h),
+             static_cast<const uint8_t *>(a.dh)},
+            {a.ld_dy * sizeof(T), a.ld_h * sizeof(T), a.ld_dh * sizeof(T)},
+            a.dh != nullptr ? 3 : 2,
+            static_cast<uint32_t>(a.cols * sizeof(T)),
+            rows_mem,
+            full};
+    ring.start(a.rows);
+  }
+  const Weight<W, NV> weight(a.weight, a.w_vec, a.cols);
   float dw[NV][8] = {};
-  int turn = 0;
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+  int it = 0;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
+    const auto load = [&](int k, const void *p, size_t ld, int col, int n, bool vec) {
+      if constexpr (kRing) return b128::load8(ring.row<T>(it, k) + col);
+      else return b128::load8_edge(static_cast<const T *>(p) + (size_t)row * ld + col, n, vec);
+    };
     const float rstd = a.rstd[row];
-    float g[NV][8], u[NV][8];  // dy * w and h * rstd
     float along = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      Raw8<T> rd{}, rh{};
-      Raw8<W> rw{};
-      if (n > 0) {
-        rd = b128::load8_edge(dy + (size_t)row * a.ld_dy + col, n, a.dy_vec);
-        rh = b128::load8_edge(h + (size_t)row * a.ld_h + col, n, a.h_vec);
-        rw = b128::load8_edge(w + col, n, a.w_vec);
-      }
-      float wv[8];
-      b128::unpack(rd, g[i]);
-      b128::unpack(rh, u[i]);
-      b128::unpack(rw, wv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u[i][j] = j < n ? u[i][j] * rstd : 0.0f;
-        dw[i][j] = fmaf(g[i][j], u[i][j], dw[i][j]);
-        g[i][j] *= wv[j];
-        along = fmaf(g[i][j], u[i][j], along);
-      }
-    }
-    const float mean = cta_sum(along, part[turn]) / static_cast<float>(a.cols);
+    if constexpr (kRing) ring.wait(it);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
       if (n <= 0) continue;
-      float v[8], past[8] = {};
-      if (dh != nullptr)
-        b128::unpack(b128::load8_edge(dh + (size_t)row * a.ld_dh + col, n, a.dh_vec), past);
+      float g[8], u[8], wv[8];
+      b128::unpack(load(0, a.dy, a.ld_dy, col, n, a.dy_vec), g);
+      b128::unpack(load(1, a.h, a.ld_h, col, n, a.h_vec), u);
+      b128::unpack(weight.chunk(i, col, n), wv);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fmaf(rstd, g[i][j] - u[i][j] * mean, past[j]);
+      for (int j = 0; j < 8; ++j) {
+        // behind the row's end: not 0 * inf, which would be NaN
+        const float unit = j < n ? u[j] * rstd : 0.0f;
+        dw[i][j] = fmaf(g[j], unit, dw[i][j]);
+        along = fmaf(g[j] * wv[j], unit, along);
+      }
+    }
+    const float mean = cta_sum(along, part[it & 1]) / static_cast<float>(a.cols);
+    // every thread is past the last row: its place takes another
+    if constexpr (kRing)
+      if (threadIdx.x == 0 && it > 0) ring.load(it - 1 + kStages, a.rows);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
+      if (n <= 0) continue;
+      float g[8], u[8], wv[8], past[8] = {};
+      b128::unpack(load(0, a.dy, a.ld_dy, col, n, a.dy_vec), g);
+      b128::unpack(load(1, a.h, a.ld_h, col, n, a.h_vec), u);
+      if (a.dh != nullptr) b128::unpack(load(2, a.dh, a.ld_dh, col, n, a.dh_vec), past);
+      b128::unpack(weight.chunk(i, col, n), wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        g[j] = fmaf(rstd, g[j] * wv[j] - u[j] * rstd * mean, past[j]);
       Raw8<T> out;
-      b128::pack(v, out);
+      b128::pack(g, out);
       b128::store8_edge(static_cast<T *>(a.dx) + (size_t)row * a.ld_dx + col, out, n, a.dx_vec);
     }
   }
@@ -182,53 +319,111 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_back(const NormBackArgs a) {
   }
 }
 
-// dweight[c] = sum of the partial rows, in their order.
-__global__ void k_sum_parts(const float *__restrict__ parts, size_t ld, int n, int cols,
-                            float *__restrict__ out) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= cols) return;
+// dweight[c] = sum of the partial rows: 32 columns a CTA, 32 threads take
+// every 32nd row each, in order, and their sums are added in a tree.
+__global__ void __launch_bounds__(1024) k_sum_parts(const float *__restrict__ parts, size_t ld,
+                                                    int n, int cols, float *__restrict__ out) {
+  __shared__ float sums[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
   float s = 0.0f;
-  for (int r = 0; r < n; ++r) s += parts[(size_t)r * ld + c];
-  out[c] = s;
-}
-
-int back_ctas(int rows) {
-  const int most = current_sm_count() * 2;
-  const int ctas = rows < most ? rows : most;
-  return ctas < kMaxParts ? ctas : kMaxParts;
+  if (c < cols) {
+#pragma unroll 8
+    for (int r = threadIdx.y; r < n; r += 32) s += parts[(size_t)r * ld + c];
+  }
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = sums[threadIdx.x][threadIdx.y];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int at = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && at < cols) out[at] = s;
 }
 
 size_t parts_pitch(int cols) { return ((size_t)cols + 63) / 64 * 64; }
 
-// Threads that hold `cols` in NV chunks of 8 each.
+// Chunks of 8 columns a thread, and threads (at most 1024) that hold a row.
+int chunks_for(int cols) { return cols <= 4096 ? 1 : cols <= 16384 ? 2 : 4; }
+
 int threads_for(int cols, int nv) {
   const int chunks = (cols + 7) / 8;
   const int t = (chunks + nv - 1) / nv;
   return (t + 31) / 32 * 32;
 }
 
-int chunks_for(int cols) { return cols <= 8192 ? 1 : cols <= 16384 ? 2 : 4; }
-
-template <typename T, typename W>
-int launch_norm(const NormArgs &a, cudaStream_t stream) {
-  const int nv = chunks_for(a.cols), threads = threads_for(a.cols, nv);
-  const int most = current_sm_count() * (2048 / threads);
-  const int grid = a.rows < most ? a.rows : most;
-  if (nv == 1) k_rmsnorm<T, W, 1><<<grid, threads, 0, stream>>>(a);
-  else if (nv == 2) k_rmsnorm<T, W, 2><<<grid, threads, 0, stream>>>(a);
-  else k_rmsnorm<T, W, 4><<<grid, threads, 0, stream>>>(a);
-  CMB_LAUNCH_CHECK();
+template <typename A>
+int launch_rows(void (*kernel)(A), const A &a, int grid, int threads, size_t smem,
+                cudaStream_t stream) {
+  if (smem > 48 * 1024)
+    CMB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(smem)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CMB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   return CMB_OK;
 }
 
+// How many CTAs walk over the rows: what fits on the device at once, with 64
+// registers a thread and `smem` bytes a CTA.
+int ctas_for(int rows, int threads, size_t smem) {
+  int fit = 1024 / threads;
+  const int by_smem = static_cast<int>(220 * 1024 / (smem + 1024));
+  if (fit > by_smem) fit = by_smem;
+  if (fit > 32) fit = 32;
+  const int most = current_sm_count() * (fit > 0 ? fit : 1);
+  return rows < most ? rows : most;
+}
+
+constexpr size_t kRingMost = 200 * 1024;
+
+template <typename T, typename W, int NV>
+int launch_norm(const NormArgs &a, cudaStream_t stream) {
+  const int threads = threads_for(a.cols, NV), direct = ctas_for(a.rows, threads, 0);
+  const size_t ring = (size_t)kStages * a.cols * sizeof(T) * (a.residual != nullptr ? 2 : 1);
+  if (a.rows > direct && a.cols % 8 == 0 && a.x_vec && (a.residual == nullptr || a.r_vec) &&
+      ring <= kRingMost)
+    return launch_rows(k_rmsnorm<T, W, NV, true>, a, ctas_for(a.rows, threads, ring), threads,
+                       ring, stream);
+  return launch_rows(k_rmsnorm<T, W, NV, false>, a, direct, threads, 0, stream);
+}
+
 template <typename T, typename W>
-int launch_back(const NormBackArgs &a, int grid, cudaStream_t stream) {
-  const int nv = chunks_for(a.cols), threads = threads_for(a.cols, nv);
-  if (nv == 1) k_rmsnorm_back<T, W, 1><<<grid, threads, 0, stream>>>(a);
-  else if (nv == 2) k_rmsnorm_back<T, W, 2><<<grid, threads, 0, stream>>>(a);
-  else k_rmsnorm_back<T, W, 4><<<grid, threads, 0, stream>>>(a);
-  CMB_LAUNCH_CHECK();
-  return CMB_OK;
+int launch_norm(const NormArgs &a, cudaStream_t stream) {
+  switch (chunks_for(a.cols)) {
+    case 1: return launch_norm<T, W, 1>(a, stream);
+    case 2: return launch_norm<T, W, 2>(a, stream);
+    default: return launch_norm<T, W, 4>(a, stream);
+  }
+}
+
+template <typename T, typename W, int NV>
+int launch_back(NormBackArgs a, int *grid, cudaStream_t stream) {
+  const int threads = threads_for(a.cols, NV), direct = ctas_for(a.rows, threads, 0);
+  const size_t ring = (size_t)kStages * a.cols * sizeof(T) * (a.dh != nullptr ? 3 : 2);
+  const bool use_ring = a.rows > direct && a.cols % 8 == 0 && a.dy_vec && a.h_vec &&
+                        (a.dh == nullptr || a.dh_vec) && ring <= kRingMost;
+  *grid = use_ring ? ctas_for(a.rows, threads, ring) : direct;
+  if (*grid > kMaxParts) *grid = kMaxParts;
+  if (use_ring) return launch_rows(k_rmsnorm_back<T, W, NV, true>, a, *grid, threads, ring, stream);
+  return launch_rows(k_rmsnorm_back<T, W, NV, false>, a, *grid, threads, 0, stream);
+}
+
+template <typename T, typename W>
+int launch_back(const NormBackArgs &a, int *grid, cudaStream_t stream) {
+  switch (chunks_for(a.cols)) {
+    case 1: return launch_back<T, W, 1>(a, grid, stream);
+    case 2: return launch_back<T, W, 2>(a, grid, stream);
+    default: return launch_back<T, W, 4>(a, grid, stream);
+  }
 }
 
 // A matrix operand of a norm: its name, address, pitch and whether it has to
@@ -362,15 +557,24 @@ extern "C" int cmb_rmsnorm_backward(const void *dy, size_t ld_dy, const void *h,
   a.dh_vec = b128::aligned_to(dh, ld_dh * elem, 16);
   a.w_vec = b128::aligned_to(weight, 0, 16);
   a.dx_vec = b128::aligned_to(dx, ld_dx * elem, 16);
-  const int grid = back_ctas(rows);
+  int grid = 0;
   if (type == CMB_BF16)
-    rc = weight_type == CMB_BF16 ? launch_back<__nv_bfloat16, __nv_bfloat16>(a, grid, stream)
-                                 : launch_back<__nv_bfloat16, float>(a, grid, stream);
+    rc = weight_type == CMB_BF16 ? launch_back<__nv_bfloat16, __nv_bfloat16>(a, &grid, stream)
+                                 : launch_back<__nv_bfloat16, float>(a, &grid, stream);
   else
-    rc = weight_type == CMB_BF16 ? launch_back<float, __nv_bfloat16>(a, grid, stream)
-                                 : launch_back<float, float>(a, grid, stream);
+    rc = weight_type == CMB_BF16 ? launch_back<float, __nv_bfloat16>(a, &grid, stream)
+                                 : launch_back<float, float>(a, &grid, stream);
   if (rc || dweight == nullptr) return rc;
-  k_sum_parts<<<(cols + 127) / 128, 128, 0, stream>>>(a.parts, a.ld_parts, grid, cols, dweight);
-  CMB_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((cols + 31) / 32);
+  cfg.blockDim = dim3(32, 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CMB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_sum_parts, static_cast<const float *>(a.parts),
+                                  a.ld_parts, grid, cols, dweight));
   return CMB_OK;
 }
