@@ -156,6 +156,43 @@ __device__ __forceinline__ uint32_t top_bits(const Raw8<float> &r) {
              max(max(r.b.x & m, r.b.y & m), max(r.b.z & m, r.b.w & m)));
 }
 
+// The same for each row and each column of 8 x 8 values.
+__device__ __forceinline__ void tops(const Raw8<__nv_bfloat16> (&r)[8], uint32_t (&rmax)[8],
+                                     uint32_t (&cmax)[8]) {
+  uint32_t c[4] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w[4] = {r[i].a.x & 0x7FFF7FFFu, r[i].a.y & 0x7FFF7FFFu, r[i].a.z & 0x7FFF7FFFu,
+                           r[i].a.w & 0x7FFF7FFFu};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] = __vmaxu2(c[k], w[k]);
+    const uint32_t v = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+    rmax[i] = max(v << 16, v & 0xFFFF0000u);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    cmax[2 * k] = c[k] << 16;
+    cmax[2 * k + 1] = c[k] & 0xFFFF0000u;
+  }
+}
+__device__ __forceinline__ void tops(const Raw8<float> (&r)[8], uint32_t (&rmax)[8],
+                                     uint32_t (&cmax)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) cmax[j] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w[8] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w,
+                           r[i].b.x, r[i].b.y, r[i].b.z, r[i].b.w};
+    rmax[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t m = w[j] & 0x7FFFFFFFu;
+      rmax[i] = max(rmax[i], m);
+      cmax[j] = max(cmax[j], m);
+    }
+  }
+}
+
 __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&v);

@@ -4,7 +4,10 @@
 //
 //   e = smallest integer with max|x| / 2^e <= 448,  q = e4m3(x * 2^-e)
 //
-// Memory bound: 2 or 4 bytes read and 1 or 2 written for each value.
+// Memory bound: 2 or 4 bytes read and 1 or 2 written for each value.  Maxima
+// are taken on the values' bits, two bf16 an instruction; whether a block has
+// anything that is not finite shows in its maximum, and only tiles that do
+// take the path that looks at each value.
 #include "block128.cuh"
 #include "cmb_host.h"
 
@@ -12,6 +15,7 @@ namespace cmb {
 namespace {
 
 using b128::kBlock;
+using b128::Raw8;
 
 struct QuantArgs {
   const void *src;
@@ -22,118 +26,257 @@ struct QuantArgs {
   bool src_vec, dst_vec, dst_t_vec;  // 16-byte loads, 8-byte stores
 };
 
+// Rows alone (blocks of 1 x 128, no transpose): 16 lanes a block, 8 values a
+// lane, two blocks a thread in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) k_quantize_rows(const QuantArgs a) {
+  constexpr int kUnroll = 2;
+  const T *src = static_cast<const T *>(a.src);
+  const int groups = b128::groups_of(a.cols);
+  const int lane16 = threadIdx.x & 15;
+  const long long half_warps = (long long)gridDim.x * (blockDim.x / 16);
+  const long long total = (long long)a.rows * groups;
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
+  // warp-uniform bound: both halves of a warp take part in the shuffles
+  const long long me = (long long)blockIdx.x * (blockDim.x / 16) + threadIdx.x / 16;
+  for (long long base = me & ~1LL; base < total; base += half_warps * kUnroll) {
+    Raw8<T> raw[kUnroll];
+    long long at[kUnroll];
+    int row[kUnroll], group[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      at[u] = base + (me & 1) + u * half_warps;
+      row[u] = static_cast<int>(at[u] / groups);
+      group[u] = static_cast<int>(at[u] - (long long)row[u] * groups);
+      const int col = group[u] * kBlock + lane16 * 8;
+      raw[u] = {};
+      if (at[u] < total && col < a.cols)
+        raw[u] = b128::load8_edge(src + (size_t)row[u] * a.ld_src + col, a.cols - col, a.src_vec);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      uint32_t top = b128::top_bits(raw[u]);
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float v[8];
+      b128::unpack(raw[u], v);
+      const bool any = __any_sync(0xffffffffu, top >= b128::kInfBits);
+      if (any) {
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, b128::finite_magnitude(v[j]));
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        top = __float_as_uint(m);
+      }
+      const uint32_t byte = b128::scale_byte(__uint_as_float(top));
+      const float inv = b128::scale_reciprocal(byte);
+      const int col = group[u] * kBlock + lane16 * 8;
+      if (at[u] < total && col < a.cols) {
+        b128::store_bytes(a.dst + (size_t)row[u] * a.ld_dst + col,
+                          any ? b128::e4m3x8<true>(v, inv) : b128::e4m3x8<false>(v, inv),
+                          a.cols - col, a.dst_vec);
+        if (lane16 == 0)
+          a.scale[(size_t)row[u] * a.ld_scale + group[u]] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
+// What a thread of a tile holds: 8 rows x 8 columns.
+template <typename T>
+struct Piece {
+  Raw8<T> raw[8];
+  int row, col, nrow, ncol;  // in the matrix; how much of it is there
+};
+
+// Column j of the piece, rows downwards.
+__device__ __forceinline__ void column(const Piece<__nv_bfloat16> &p, int j, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w = j < 2   ? p.raw[i].a.x
+                       : j < 4 ? p.raw[i].a.y
+                       : j < 6 ? p.raw[i].a.z
+                               : p.raw[i].a.w;
+    v[i] = __uint_as_float((j & 1) ? w & 0xFFFF0000u : w << 16);
+  }
+}
+__device__ __forceinline__ void column(const Piece<float> &p, int j, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 w = j < 4 ? p.raw[i].a : p.raw[i].b;
+    const int k = j & 3;
+    v[i] = __uint_as_float(k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w);
+  }
+}
+
+// Writes both forms; row_inv and col_inv are the reciprocals of the scales of
+// the tile's rows and columns.
+template <bool kAny, typename T>
+__device__ __forceinline__ void store_piece(const QuantArgs &a, const Piece<T> &p,
+                                            const float *row_inv, const float *col_inv) {
+  if (a.dst != nullptr && p.ncol > 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i >= p.nrow) continue;
+      float v[8];
+      b128::unpack(p.raw[i], v);
+      b128::store_bytes(a.dst + (size_t)(p.row + i) * a.ld_dst + p.col,
+                        b128::e4m3x8<kAny>(v, row_inv[i]), p.ncol, a.dst_vec);
+    }
+  }
+  if (a.dst_t != nullptr && p.nrow > 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j >= p.ncol) continue;
+      float v[8];
+      column(p, j, v);
+      b128::store_bytes(a.dst_t + (size_t)(p.col + j) * a.ld_dst_t + p.row,
+                        b128::e4m3x8<kAny>(v, col_inv[j]), p.nrow, a.dst_t_vec);
+    }
+  }
+}
+
 // One CTA per 128 x 128 tile: a whole block of every kind, so its maxima
 // need nothing from outside.  8 warps stand 4 (columns) x 2 (rows); a thread
 // holds 8 rows x 8 columns, a warp 64 rows x 32 columns, so each row a warp
 // loads is 64 bytes (bf16) and each column it stores 64 bytes: whole 32-byte
 // sectors both ways with no trip through shared memory.
 template <typename T>
-__global__ void __launch_bounds__(256) k_quantize_tile(const QuantArgs a) {
-  __shared__ float row_part[4][kBlock], col_part[2][kBlock], all_part[8];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize_tile(const QuantArgs a) {
+  __shared__ uint32_t row_part[4][kBlock], col_part[2][kBlock];
+  __shared__ __align__(16) float row_inv[kBlock], col_inv[kBlock];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wc = warp & 3, wr = warp >> 2;
   const int lc = lane & 3, lr = lane >> 2;
   const int col_in = wc * 32 + lc * 8, row_in = wr * 64 + lr * 8;
-  const int col = blockIdx.x * kBlock + col_in;
-  const int ncol = min(8, a.cols - col);
   const T *src = static_cast<const T *>(a.src);
+  Piece<T> p;
+  p.col = blockIdx.x * kBlock + col_in;
+  p.ncol = min(8, a.cols - p.col);
+  dev::grid_dep_wait();
+  dev::grid_dep_launch();
 
   for (int tile_r = blockIdx.y; tile_r < b128::groups_of(a.rows); tile_r += gridDim.y) {
-    const int row = tile_r * kBlock + row_in;
-    b128::Raw8<T> raw[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      raw[i] = row + i < a.rows
-                   ? b128::load8_edge(src + (size_t)(row + i) * a.ld_src + col, ncol, a.src_vec)
-                   : b128::Raw8<T>{};
-    float rmax[8], cmax[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) cmax[i] = 0.0f;
+    p.row = tile_r * kBlock + row_in;
+    p.nrow = min(8, a.rows - p.row);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v[8];
-      b128::unpack(raw[i], v);
-      rmax[i] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float m = b128::finite_magnitude(v[j]);
-        rmax[i] = fmaxf(rmax[i], m);
-        cmax[j] = fmaxf(cmax[j], m);
-      }
+      p.raw[i] = {};
+      if (i < p.nrow && p.ncol > 0)
+        p.raw[i] = b128::load8_edge(src + (size_t)(p.row + i) * a.ld_src + p.col, p.ncol, a.src_vec);
     }
-    if (a.block_rows == 1) {
+    // Maxima of the piece's rows and columns, as bits; once more over the
+    // finite values alone where the tile has others.
+    bool any = false;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+      uint32_t rmax[8], cmax[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // over the 4 lanes of a row, then the 4 warps
-        rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 1));
-        rmax[i] = fmaxf(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 2));
-        if (lc == 0) row_part[wc][row_in + i] = rmax[i];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1)
-          cmax[i] = fmaxf(cmax[i], __shfl_xor_sync(0xffffffffu, cmax[i], o));
-        if (lr == 0) col_part[wr][col_in + i] = cmax[i];
-      }
-    } else {
-      float m = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, rmax[i]);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (lane == 0) all_part[warp] = m;
-    }
-    __syncthreads();
-    uint32_t rbyte[8], cbyte[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (a.block_rows == 1) {
-        const float r = fmaxf(fmaxf(row_part[0][row_in + i], row_part[1][row_in + i]),
-                              fmaxf(row_part[2][row_in + i], row_part[3][row_in + i]));
-        rbyte[i] = b128::scale_byte(r);
-        cbyte[i] = b128::scale_byte(fmaxf(col_part[0][col_in + i], col_part[1][col_in + i]));
+      for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = 0;
+      if (pass == 0) {
+        b128::tops(p.raw, rmax, cmax);
       } else {
-        float m = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, all_part[k]);
-        rbyte[i] = cbyte[i] = b128::scale_byte(m);
-      }
-    }
-    if (a.dst != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (row + i >= a.rows) continue;
-        float v[8];
-        b128::unpack(raw[i], v);
-        if (ncol > 0)
-          b128::store_bytes(a.dst + (size_t)(row + i) * a.ld_dst + col,
-                            b128::e4m3x8<true>(v, b128::scale_reciprocal(rbyte[i])), ncol, a.dst_vec);
-        if (a.block_rows == 1 && col_in == 0)
-          a.scale[(size_t)(row + i) * a.ld_scale + blockIdx.x] = static_cast<uint8_t>(rbyte[i]);
-      }
-      if (a.block_rows != 1 && threadIdx.x == 0)
-        a.scale[(size_t)tile_r * a.ld_scale + blockIdx.x] = static_cast<uint8_t>(rbyte[0]);
-    }
-    if (a.dst_t != nullptr) {
-      const int nrow = min(8, a.rows - row);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j >= ncol) continue;
-        float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float w[8];
-          b128::unpack(raw[i], w);
-          v[i] = w[j];
+          float v[8];
+          b128::unpack(p.raw[i], v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t m = __float_as_uint(b128::finite_magnitude(v[j]));
+            rmax[i] = max(rmax[i], m);
+            cmax[j] = max(cmax[j], m);
+          }
         }
-        if (nrow > 0)
-          b128::store_bytes(a.dst_t + (size_t)(col + j) * a.ld_dst_t + row,
-                            b128::e4m3x8<true>(v, b128::scale_reciprocal(cbyte[j])), nrow, a.dst_t_vec);
-        if (a.block_rows == 1 && row_in == 0)
-          a.scale_t[(size_t)(col + j) * a.ld_scale_t + tile_r] = static_cast<uint8_t>(cbyte[j]);
       }
-      if (a.block_rows != 1 && threadIdx.x == 0)
-        a.scale_t[(size_t)blockIdx.x * a.ld_scale_t + tile_r] = static_cast<uint8_t>(cbyte[0]);
+      if (a.block_rows == kBlock) {  // one maximum: rows of the piece stand for all
+#pragma unroll
+        for (int i = 1; i < 8; ++i) rmax[0] = max(rmax[0], rmax[i]);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+          rmax[0] = max(rmax[0], __shfl_xor_sync(0xffffffffu, rmax[0], o));
+        if (lane == 0) row_part[wc][wr] = rmax[0];
+      } else {
+        if (a.dst != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // over the 4 lanes of a row, then the 4 warps
+            rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 1));
+            rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 2));
+          }
+          if (lc == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row_part[wc][row_in + i] = rmax[i];
+          }
+        }
+        if (a.dst_t != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1)
+              cmax[i] = max(cmax[i], __shfl_xor_sync(0xffffffffu, cmax[i], o));
+          if (lr == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) col_part[wr][col_in + i] = cmax[i];
+          }
+        }
+      }
+      __syncthreads();
+      // thread t: row t of the tile, or column t - 128
+      const int k = threadIdx.x & 127;
+      const bool is_row = threadIdx.x < 128;
+      uint32_t top = 0;
+      if (a.block_rows == kBlock) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, row_part[i & 3][i >> 2]);
+      } else if (is_row && a.dst != nullptr) {
+        top = max(max(row_part[0][k], row_part[1][k]), max(row_part[2][k], row_part[3][k]));
+      } else if (!is_row && a.dst_t != nullptr) {
+        top = max(col_part[0][k], col_part[1][k]);
+      }
+      const uint32_t byte = b128::scale_byte(__uint_as_float(top));
+      (is_row ? row_inv : col_inv)[k] = b128::scale_reciprocal(byte);
+      if (pass == 0) {
+        any = __syncthreads_or(top >= b128::kInfBits);
+        if (any) continue;
+      } else {
+        __syncthreads();
+      }
+      const int tall = a.block_rows == 1 ? 1 : kBlock;  // rows that share a scale
+      const int r = tile_r * kBlock + k, c = blockIdx.x * kBlock + k;
+      if (is_row && a.dst != nullptr && r < a.rows && k % tall == 0)
+        a.scale[(size_t)(r / tall) * a.ld_scale + blockIdx.x] = static_cast<uint8_t>(byte);
+      if (!is_row && a.dst_t != nullptr && c < a.cols && k % tall == 0)
+        a.scale_t[(size_t)(c / tall) * a.ld_scale_t + tile_r] = static_cast<uint8_t>(byte);
+      break;
     }
-    __syncthreads();  // the maxima are read before the next tile writes them
+    if (any) store_piece<true>(a, p, row_inv + row_in, col_inv + col_in);
+    else store_piece<false>(a, p, row_inv + row_in, col_inv + col_in);
+    __syncthreads();  // the reciprocals are read before the next tile writes them
   }
+}
+
+template <typename T>
+int launch_quantize(const QuantArgs &a, cudaStream_t stream) {
+  const int tiles_c = b128::groups_of(a.cols), tiles_r = b128::groups_of(a.rows);
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (a.block_rows == 1 && a.dst_t == nullptr) {
+    const long long ctas = ((long long)a.rows * tiles_c + 31) / 32;  // 16 blocks a CTA, twice
+    const long long most = (long long)current_sm_count() * 8;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas < most ? ctas : most));
+    CMB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_quantize_rows<T>, a));
+    return CMB_OK;
+  }
+  cfg.gridDim = dim3(tiles_c, tiles_r < 65535 ? tiles_r : 65535);
+  CMB_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_quantize_tile<T>, a));
+  return CMB_OK;
 }
 
 }  // namespace
@@ -173,12 +316,6 @@ extern "C" int cmb_quantize_e4m3_block128(const void *src, int src_type, int row
   a.src_vec = b128::aligned_to(src, ld_src * elem, 16);
   a.dst_vec = b128::aligned_to(dst, ld_dst, 8);
   a.dst_t_vec = b128::aligned_to(dst_t, ld_dst_t, 8);
-  const int tiles_c = b128::groups_of(cols), tiles_r = b128::groups_of(rows);
-  const dim3 grid(tiles_c, tiles_r < 65535 ? tiles_r : 65535);
-  if (src_type == CMB_BF16)
-    k_quantize_tile<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
-  else
-    k_quantize_tile<float><<<grid, 256, 0, stream>>>(a);
-  CMB_LAUNCH_CHECK();
-  return CMB_OK;
+  return src_type == CMB_BF16 ? launch_quantize<__nv_bfloat16>(a, stream)
+                              : launch_quantize<float>(a, stream);
 }

@@ -23,7 +23,10 @@ namespace {
 using b128::Raw8;
 
 constexpr int kMaxParts = 1024;  // rows of partial weight gradients in the workspace
-constexpr int kStages = 3;       // rows in the ring
+// Rows in the ring.  Two leave room for two CTAs of a wide row on a SM, which
+// counts for more than depth: the backward pass of 8192 x 8192 bf16 takes 90 us
+// with two, 108 with three or four (one CTA a SM); the norm 81, 80 and 102.
+constexpr int kStages = 2;
 
 // Sum over the CTA, the same value in every thread.  `part` holds one float
 // for each warp; two calls in a row use different ones.
