@@ -244,15 +244,14 @@ __device__ __forceinline__ void store8_edge(T *p, const Raw8<T> &r, int n, bool 
     if (i < n) p[i] = from_float<T>(v[i]);
 }
 
-// 8 bytes, or the first n of them.
+// 8 bytes, or the first n of them; the odd case out of the way of the other.
+static __device__ __noinline__ void store_bytes_edge(uint8_t *p, uint2 q, int n) {
+  for (int i = 0; i < 8 && i < n; ++i)
+    p[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+}
 __device__ __forceinline__ void store_bytes(uint8_t *p, uint2 q, int n, bool aligned) {
-  if (aligned && n >= 8) {
-    *reinterpret_cast<uint2 *>(p) = q;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+  if (aligned && n >= 8) *reinterpret_cast<uint2 *>(p) = q;
+  else store_bytes_edge(p, q, n);
 }
 
 // ------------------------------------------------------------ host checks

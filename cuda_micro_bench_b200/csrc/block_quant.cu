@@ -88,52 +88,97 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const QuantArgs a) {
 template <typename T>
 struct Piece {
   Raw8<T> raw[8];
-  int row, col, nrow, ncol;  // in the matrix; how much of it is there
+  int row, col, nrow, ncol;  // in the matrix; how much of it is there (up to 8)
 };
 
-// Column j of the piece, rows downwards.
-__device__ __forceinline__ void column(const Piece<__nv_bfloat16> &p, int j, float (&v)[8]) {
+// 8 x 8 values to e4m3: rows[i] = row i by its scale, cols[j] = column j, rows
+// downwards, by its own.  bf16 values are multiplied by the powers of two in
+// bf16, two at a time: exact, but for results under 2^-126, which are zeros in
+// e4m3 either way.
+template <bool kAny>
+__device__ __forceinline__ uint2 row_bytes(const Raw8<__nv_bfloat16> &r, float inv) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+  const __nv_bfloat162 s = __float2bfloat162_rn(inv);
+  uint32_t h[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t w = j < 2   ? p.raw[i].a.x
-                       : j < 4 ? p.raw[i].a.y
-                       : j < 6 ? p.raw[i].a.z
-                               : p.raw[i].a.w;
-    v[i] = __uint_as_float((j & 1) ? w & 0xFFFF0000u : w << 16);
+  for (int k = 0; k < 4; ++k) {
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w[k]), s);
+    const uint32_t u = *reinterpret_cast<const uint32_t *>(&v);
+    h[k] = b128::e4m3x2<kAny>(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
-__device__ __forceinline__ void column(const Piece<float> &p, int j, float (&v)[8]) {
+template <bool kAny>
+__device__ __forceinline__ uint2 row_bytes(const Raw8<float> &r, float inv) {
+  float v[8];
+  b128::unpack(r, v);
+  return b128::e4m3x8<kAny>(v, inv);
+}
+
+// Columns 2 k and 2 k + 1 of the piece.
+template <bool kAny>
+__device__ __forceinline__ void column_bytes(const Raw8<__nv_bfloat16> (&raw)[8], int k, float inv0,
+                                             float inv1, uint2 (&q)[2]) {
+  const __nv_bfloat162 s = __floats2bfloat162_rn(inv0, inv1);
+  uint32_t h[2][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4 w = j < 4 ? p.raw[i].a : p.raw[i].b;
-    const int k = j & 3;
-    v[i] = __uint_as_float(k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w);
+  for (int i = 0; i < 8; i += 2) {
+    uint32_t u[2];
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const uint4 r = raw[i + d].a;
+      const uint32_t w = k == 0 ? r.x : k == 1 ? r.y : k == 2 ? r.z : r.w;
+      const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w), s);
+      u[d] = *reinterpret_cast<const uint32_t *>(&v);
+    }
+    h[0][i / 2] = b128::e4m3x2<kAny>(__uint_as_float(u[0] << 16), __uint_as_float(u[1] << 16));
+    h[1][i / 2] = b128::e4m3x2<kAny>(__uint_as_float(u[0] & 0xFFFF0000u),
+                                     __uint_as_float(u[1] & 0xFFFF0000u));
+  }
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+    q[d] = make_uint2(h[d][0] | (h[d][1] << 16), h[d][2] | (h[d][3] << 16));
+}
+template <bool kAny>
+__device__ __forceinline__ void column_bytes(const Raw8<float> (&raw)[8], int k, float inv0,
+                                             float inv1, uint2 (&q)[2]) {
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 r = k < 2 ? raw[i].a : raw[i].b;
+      const int at = 2 * (k & 1) + d;
+      v[i] = __uint_as_float(at == 0 ? r.x : at == 1 ? r.y : at == 2 ? r.z : r.w);
+    }
+    q[d] = b128::e4m3x8<kAny>(v, d == 0 ? inv0 : inv1);
   }
 }
 
 // Writes both forms; row_inv and col_inv are the reciprocals of the scales of
-// the tile's rows and columns.
+// the piece's rows and columns.
 template <bool kAny, typename T>
 __device__ __forceinline__ void store_piece(const QuantArgs &a, const Piece<T> &p,
                                             const float *row_inv, const float *col_inv) {
   if (a.dst != nullptr && p.ncol > 0) {
+    uint8_t *to = a.dst + (size_t)p.row * a.ld_dst + p.col;
+    const bool vec = a.dst_vec && p.ncol == 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= p.nrow) continue;
-      float v[8];
-      b128::unpack(p.raw[i], v);
-      b128::store_bytes(a.dst + (size_t)(p.row + i) * a.ld_dst + p.col,
-                        b128::e4m3x8<kAny>(v, row_inv[i]), p.ncol, a.dst_vec);
+    for (int i = 0; i < 8; ++i, to += a.ld_dst) {
+      const uint2 q = row_bytes<kAny>(p.raw[i], row_inv[i]);
+      if (i < p.nrow) b128::store_bytes(to, q, p.ncol, vec);
     }
   }
   if (a.dst_t != nullptr && p.nrow > 0) {
+    uint8_t *to = a.dst_t + (size_t)p.col * a.ld_dst_t + p.row;
+    const bool vec = a.dst_t_vec && p.nrow == 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j >= p.ncol) continue;
-      float v[8];
-      column(p, j, v);
-      b128::store_bytes(a.dst_t + (size_t)(p.col + j) * a.ld_dst_t + p.row,
-                        b128::e4m3x8<kAny>(v, col_inv[j]), p.nrow, a.dst_t_vec);
+    for (int k = 0; k < 4; ++k) {
+      uint2 q[2];
+      column_bytes<kAny>(p.raw, k, col_inv[2 * k], col_inv[2 * k + 1], q);
+#pragma unroll
+      for (int d = 0; d < 2; ++d, to += a.ld_dst_t)
+        if (2 * k + d < p.ncol) b128::store_bytes(to, q[d], p.nrow, vec);
     }
   }
 }
