@@ -51,17 +51,25 @@ __device__ __forceinline__ uint32_t magnitude_bits(float x) {
   return __float_as_uint(x) & 0x7FFFFFFFu;
 }
 
-// Two values to e4m3 (nearest even), `lo` in the low byte.  The scale keeps
-// finite values within 448, so saturation only ever meets infinities; where a
-// block may hold any (kAny), those become NaN, as NaN does.
+// Four values to e4m3 (nearest even), the first in the low byte.  The scale
+// keeps finite values within 448, so saturation only ever meets infinities;
+// where a block may hold any (kAny), those become NaN, as NaN does.
 template <bool kAny>
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  uint32_t v = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  uint32_t q;
+  asm("{ .reg .b16 l, h;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+      "mov.b32 %0, {l, h}; }"
+      : "=r"(q)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
   if constexpr (kAny) {
-    if (!(fabsf(lo) <= kMaxFinite)) v = (v & 0xFF00u) | 0x7Fu;
-    if (!(fabsf(hi) <= kMaxFinite)) v = (v & 0x00FFu) | 0x7F00u;
+    const float v[4] = {a, b, c, d};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(fabsf(v[i]) <= kMaxFinite)) q = (q & ~(0xFFu << (8 * i))) | (0x7Fu << (8 * i));
   }
-  return v;
+  return q;
 }
 
 // a * s, both halves at once.
@@ -81,13 +89,26 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 s) {
 template <bool kAny>
 __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
   const float2 s = make_float2(inv, inv);
-  uint32_t h[4];
+  float2 p[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = mul2(make_float2(v[2 * i], v[2 * i + 1]), s);
-    h[i] = e4m3x2<kAny>(p.x, p.y);
-  }
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+  for (int i = 0; i < 4; ++i) p[i] = mul2(make_float2(v[2 * i], v[2 * i + 1]), s);
+  return make_uint2(e4m3x4<kAny>(p[0].x, p[0].y, p[1].x, p[1].y),
+                    e4m3x4<kAny>(p[2].x, p[2].y, p[3].x, p[3].y));
+}
+
+// Both bf16 halves of a word times a bf16 each (given as fp32 bits' upper
+// half), in fp32: one instruction a value, with no unpacking.
+__device__ __forceinline__ float2 mul_bf16x2(uint32_t w, uint32_t lo_scale, uint32_t hi_scale) {
+  float2 r;
+  asm("{ .reg .b16 l, h, s, t, x;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "mov.b32 {x, s}, %3;\n\t"
+      "mov.b32 {x, t}, %4;\n\t"
+      "fma.rn.f32.bf16 %0, l, s, %5;\n\t"
+      "fma.rn.f32.bf16 %1, h, t, %5; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(w), "r"(lo_scale), "r"(hi_scale), "f"(-0.0f));
+  return r;
 }
 
 // ------------------------------------------------- rows of bf16 or fp32
@@ -143,11 +164,16 @@ __device__ __forceinline__ void unpack(const Raw8<float> &r, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
 }
 
+// The larger magnitudes of two pairs of bf16; NaN wins.
+__device__ __forceinline__ uint32_t max_magnitude2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 v = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162 *>(&a)),
+                                       __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&b)));
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 // Largest magnitude's bits (as fp32 bits) of the 8; NaN and infinities count.
 __device__ __forceinline__ uint32_t top_bits(const Raw8<__nv_bfloat16> &r) {
-  const uint32_t m = 0x7FFF7FFFu;
-  const uint32_t v =
-      __vmaxu2(__vmaxu2(r.a.x & m, r.a.y & m), __vmaxu2(r.a.z & m, r.a.w & m));
+  const uint32_t v = max_magnitude2(max_magnitude2(r.a.x, r.a.y), max_magnitude2(r.a.z, r.a.w));
   return max(v << 16, v & 0xFFFF0000u);
 }
 __device__ __forceinline__ uint32_t top_bits(const Raw8<float> &r) {
@@ -162,11 +188,10 @@ __device__ __forceinline__ void tops(const Raw8<__nv_bfloat16> (&r)[8], uint32_t
   uint32_t c[4] = {};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t w[4] = {r[i].a.x & 0x7FFF7FFFu, r[i].a.y & 0x7FFF7FFFu, r[i].a.z & 0x7FFF7FFFu,
-                           r[i].a.w & 0x7FFF7FFFu};
+    const uint32_t w[4] = {r[i].a.x, r[i].a.y, r[i].a.z, r[i].a.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) c[k] = __vmaxu2(c[k], w[k]);
-    const uint32_t v = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+    for (int k = 0; k < 4; ++k) c[k] = max_magnitude2(c[k], w[k]);
+    const uint32_t v = max_magnitude2(max_magnitude2(w[0], w[1]), max_magnitude2(w[2], w[3]));
     rmax[i] = max(v << 16, v & 0xFFFF0000u);
   }
 #pragma unroll

@@ -26,6 +26,22 @@ struct QuantArgs {
   bool src_vec, dst_vec, dst_t_vec;  // 16-byte loads, 8-byte stores
 };
 
+// 8 values to e4m3, by the reciprocal of their scale.
+template <bool kAny>
+__device__ __forceinline__ uint2 row_bytes(const Raw8<__nv_bfloat16> &r, float inv) {
+  const uint32_t s = __float_as_uint(inv);
+  const float2 a = b128::mul_bf16x2(r.a.x, s, s), b = b128::mul_bf16x2(r.a.y, s, s),
+               c = b128::mul_bf16x2(r.a.z, s, s), d = b128::mul_bf16x2(r.a.w, s, s);
+  return make_uint2(b128::e4m3x4<kAny>(a.x, a.y, b.x, b.y),
+                    b128::e4m3x4<kAny>(c.x, c.y, d.x, d.y));
+}
+template <bool kAny>
+__device__ __forceinline__ uint2 row_bytes(const Raw8<float> &r, float inv) {
+  float v[8];
+  b128::unpack(r, v);
+  return b128::e4m3x8<kAny>(v, inv);
+}
+
 // Rows alone (blocks of 1 x 128, no transpose): 16 lanes a block, 8 values a
 // lane, two blocks a thread in flight.
 template <typename T>
@@ -59,11 +75,10 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const QuantArgs a) {
       uint32_t top = b128::top_bits(raw[u]);
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      float v[8];
-      b128::unpack(raw[u], v);
       const bool any = __any_sync(0xffffffffu, top >= b128::kInfBits);
       if (any) {
-        float m = 0.0f;
+        float v[8], m = 0.0f;
+        b128::unpack(raw[u], v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, b128::finite_magnitude(v[j]));
 #pragma unroll
@@ -75,7 +90,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const QuantArgs a) {
       const int col = group[u] * kBlock + lane16 * 8;
       if (at[u] < total && col < a.cols) {
         b128::store_bytes(a.dst + (size_t)row[u] * a.ld_dst + col,
-                          any ? b128::e4m3x8<true>(v, inv) : b128::e4m3x8<false>(v, inv),
+                          any ? row_bytes<true>(raw[u], inv) : row_bytes<false>(raw[u], inv),
                           a.cols - col, a.dst_vec);
         if (lane16 == 0)
           a.scale[(size_t)row[u] * a.ld_scale + group[u]] = static_cast<uint8_t>(byte);
@@ -91,53 +106,21 @@ struct Piece {
   int row, col, nrow, ncol;  // in the matrix; how much of it is there (up to 8)
 };
 
-// 8 x 8 values to e4m3: rows[i] = row i by its scale, cols[j] = column j, rows
-// downwards, by its own.  bf16 values are multiplied by the powers of two in
-// bf16, two at a time: exact, but for results under 2^-126, which are zeros in
-// e4m3 either way.
-template <bool kAny>
-__device__ __forceinline__ uint2 row_bytes(const Raw8<__nv_bfloat16> &r, float inv) {
-  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-  const __nv_bfloat162 s = __float2bfloat162_rn(inv);
-  uint32_t h[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w[k]), s);
-    const uint32_t u = *reinterpret_cast<const uint32_t *>(&v);
-    h[k] = b128::e4m3x2<kAny>(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
-  }
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-}
-template <bool kAny>
-__device__ __forceinline__ uint2 row_bytes(const Raw8<float> &r, float inv) {
-  float v[8];
-  b128::unpack(r, v);
-  return b128::e4m3x8<kAny>(v, inv);
-}
-
-// Columns 2 k and 2 k + 1 of the piece.
+// Columns 2 k and 2 k + 1 of the piece, rows downwards, each by its own.
 template <bool kAny>
 __device__ __forceinline__ void column_bytes(const Raw8<__nv_bfloat16> (&raw)[8], int k, float inv0,
                                              float inv1, uint2 (&q)[2]) {
-  const __nv_bfloat162 s = __floats2bfloat162_rn(inv0, inv1);
-  uint32_t h[2][4];
+  float2 v[8];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    uint32_t u[2];
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      const uint4 r = raw[i + d].a;
-      const uint32_t w = k == 0 ? r.x : k == 1 ? r.y : k == 2 ? r.z : r.w;
-      const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w), s);
-      u[d] = *reinterpret_cast<const uint32_t *>(&v);
-    }
-    h[0][i / 2] = b128::e4m3x2<kAny>(__uint_as_float(u[0] << 16), __uint_as_float(u[1] << 16));
-    h[1][i / 2] = b128::e4m3x2<kAny>(__uint_as_float(u[0] & 0xFFFF0000u),
-                                     __uint_as_float(u[1] & 0xFFFF0000u));
+  for (int i = 0; i < 8; ++i) {
+    const uint4 r = raw[i].a;
+    v[i] = b128::mul_bf16x2(k == 0 ? r.x : k == 1 ? r.y : k == 2 ? r.z : r.w,
+                            __float_as_uint(inv0), __float_as_uint(inv1));
   }
-#pragma unroll
-  for (int d = 0; d < 2; ++d)
-    q[d] = make_uint2(h[d][0] | (h[d][1] << 16), h[d][2] | (h[d][3] << 16));
+  q[0] = make_uint2(b128::e4m3x4<kAny>(v[0].x, v[1].x, v[2].x, v[3].x),
+                    b128::e4m3x4<kAny>(v[4].x, v[5].x, v[6].x, v[7].x));
+  q[1] = make_uint2(b128::e4m3x4<kAny>(v[0].y, v[1].y, v[2].y, v[3].y),
+                    b128::e4m3x4<kAny>(v[4].y, v[5].y, v[6].y, v[7].y));
 }
 template <bool kAny>
 __device__ __forceinline__ void column_bytes(const Raw8<float> (&raw)[8], int k, float inv0,
@@ -156,31 +139,121 @@ __device__ __forceinline__ void column_bytes(const Raw8<float> (&raw)[8], int k,
 }
 
 // Writes both forms; row_inv and col_inv are the reciprocals of the scales of
-// the piece's rows and columns.
-template <bool kAny, typename T>
+// the piece's rows and columns.  kWhole: all of the tile is there, in aligned
+// chunks, and finite.
+template <bool kWhole, typename T>
 __device__ __forceinline__ void store_piece(const QuantArgs &a, const Piece<T> &p,
                                             const float *row_inv, const float *col_inv) {
-  if (a.dst != nullptr && p.ncol > 0) {
+  if (a.dst != nullptr && (kWhole || p.ncol > 0)) {
     uint8_t *to = a.dst + (size_t)p.row * a.ld_dst + p.col;
-    const bool vec = a.dst_vec && p.ncol == 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i, to += a.ld_dst) {
-      const uint2 q = row_bytes<kAny>(p.raw[i], row_inv[i]);
-      if (i < p.nrow) b128::store_bytes(to, q, p.ncol, vec);
+      const uint2 q = row_bytes<!kWhole>(p.raw[i], row_inv[i]);
+      if constexpr (kWhole) *reinterpret_cast<uint2 *>(to) = q;
+      else if (i < p.nrow) b128::store_bytes(to, q, p.ncol, a.dst_vec);
     }
   }
-  if (a.dst_t != nullptr && p.nrow > 0) {
+  if (a.dst_t != nullptr && (kWhole || p.nrow > 0)) {
     uint8_t *to = a.dst_t + (size_t)p.col * a.ld_dst_t + p.row;
-    const bool vec = a.dst_t_vec && p.nrow == 8;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint2 q[2];
-      column_bytes<kAny>(p.raw, k, col_inv[2 * k], col_inv[2 * k + 1], q);
+      column_bytes<!kWhole>(p.raw, k, col_inv[2 * k], col_inv[2 * k + 1], q);
 #pragma unroll
-      for (int d = 0; d < 2; ++d, to += a.ld_dst_t)
-        if (2 * k + d < p.ncol) b128::store_bytes(to, q[d], p.nrow, vec);
+      for (int d = 0; d < 2; ++d, to += a.ld_dst_t) {
+        if constexpr (kWhole) *reinterpret_cast<uint2 *>(to) = q[d];
+        else if (2 * k + d < p.ncol) b128::store_bytes(to, q[d], p.nrow, a.dst_t_vec);
+      }
     }
   }
+}
+
+struct TileShared {
+  uint32_t row_part[4][kBlock], col_part[2][kBlock];
+  float row_inv[kBlock], col_inv[kBlock];
+};
+
+// Maxima of the tile's rows and columns (or of all of it), their scales and
+// the reciprocals.  kFinite: over the bits of all values, and true if any is
+// not finite, when nothing has been written; else over the finite ones.
+template <bool kFinite, typename T>
+__device__ __forceinline__ bool tile_scales(const QuantArgs &a, const Piece<T> &p, int tile_r,
+                                            int row_in, int col_in, TileShared &sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wc = warp & 3, wr = warp >> 2, lc = lane & 3, lr = lane >> 2;
+  uint32_t rmax[8], cmax[8];
+  if constexpr (kFinite) {
+    b128::tops(p.raw, rmax, cmax);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v[8];
+      b128::unpack(p.raw[i], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t m = __float_as_uint(b128::finite_magnitude(v[j]));
+        rmax[i] = max(rmax[i], m);
+        cmax[j] = max(cmax[j], m);
+      }
+    }
+  }
+  if (a.block_rows == kBlock) {  // one maximum: rows of the piece stand for all
+#pragma unroll
+    for (int i = 1; i < 8; ++i) rmax[0] = max(rmax[0], rmax[i]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+      rmax[0] = max(rmax[0], __shfl_xor_sync(0xffffffffu, rmax[0], o));
+    if (lane == 0) sh.row_part[wc][wr] = rmax[0];
+  } else {
+    if (a.dst != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // over the 4 lanes of a row, then the 4 warps
+        rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 1));
+        rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 2));
+      }
+      if (lc == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sh.row_part[wc][row_in + i] = rmax[i];
+      }
+    }
+    if (a.dst_t != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1)
+          cmax[i] = max(cmax[i], __shfl_xor_sync(0xffffffffu, cmax[i], o));
+      if (lr == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sh.col_part[wr][col_in + i] = cmax[i];
+      }
+    }
+  }
+  __syncthreads();
+  // thread t: row t of the tile, or column t - 128
+  const int k = threadIdx.x & 127;
+  const bool is_row = threadIdx.x < 128;
+  uint32_t top = 0;
+  if (a.block_rows == kBlock) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, sh.row_part[i & 3][i >> 2]);
+  } else if (is_row && a.dst != nullptr) {
+    top = max(max(sh.row_part[0][k], sh.row_part[1][k]),
+              max(sh.row_part[2][k], sh.row_part[3][k]));
+  } else if (!is_row && a.dst_t != nullptr) {
+    top = max(sh.col_part[0][k], sh.col_part[1][k]);
+  }
+  const uint32_t byte = b128::scale_byte(__uint_as_float(top));
+  (is_row ? sh.row_inv : sh.col_inv)[k] = b128::scale_reciprocal(byte);
+  if (__syncthreads_or(top >= b128::kInfBits)) return true;
+  const int tall = a.block_rows == 1 ? 1 : kBlock;  // rows that share a scale
+  const int r = tile_r * kBlock + k, c = blockIdx.x * kBlock + k;
+  if (is_row && a.dst != nullptr && r < a.rows && k % tall == 0)
+    a.scale[(size_t)(r / tall) * a.ld_scale + blockIdx.x] = static_cast<uint8_t>(byte);
+  if (!is_row && a.dst_t != nullptr && c < a.cols && k % tall == 0)
+    a.scale_t[(size_t)(c / tall) * a.ld_scale_t + tile_r] = static_cast<uint8_t>(byte);
+  return false;
 }
 
 // One CTA per 128 x 128 tile: a whole block of every kind, so its maxima
@@ -190,113 +263,37 @@ __device__ __forceinline__ void store_piece(const QuantArgs &a, const Piece<T> &
 // sectors both ways with no trip through shared memory.
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize_tile(const QuantArgs a) {
-  __shared__ uint32_t row_part[4][kBlock], col_part[2][kBlock];
-  __shared__ __align__(16) float row_inv[kBlock], col_inv[kBlock];
+  __shared__ TileShared sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wc = warp & 3, wr = warp >> 2;
-  const int lc = lane & 3, lr = lane >> 2;
-  const int col_in = wc * 32 + lc * 8, row_in = wr * 64 + lr * 8;
+  const int col_in = (warp & 3) * 32 + (lane & 3) * 8, row_in = (warp >> 2) * 64 + (lane >> 2) * 8;
   const T *src = static_cast<const T *>(a.src);
   Piece<T> p;
   p.col = blockIdx.x * kBlock + col_in;
   p.ncol = min(8, a.cols - p.col);
+  const bool wide = (blockIdx.x + 1) * kBlock <= a.cols && a.src_vec &&
+                    (a.dst == nullptr || a.dst_vec) && (a.dst_t == nullptr || a.dst_t_vec);
   dev::grid_dep_wait();
   dev::grid_dep_launch();
 
   for (int tile_r = blockIdx.y; tile_r < b128::groups_of(a.rows); tile_r += gridDim.y) {
     p.row = tile_r * kBlock + row_in;
     p.nrow = min(8, a.rows - p.row);
+    const T *from = src + (size_t)p.row * a.ld_src + p.col;
+    const bool whole = wide && (tile_r + 1) * kBlock <= a.rows;
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p.raw[i] = {};
-      if (i < p.nrow && p.ncol > 0)
-        p.raw[i] = b128::load8_edge(src + (size_t)(p.row + i) * a.ld_src + p.col, p.ncol, a.src_vec);
+      for (int i = 0; i < 8; ++i, from += a.ld_src) p.raw[i] = b128::load8(from);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i, from += a.ld_src) {
+        p.raw[i] = {};
+        if (i < p.nrow && p.ncol > 0) p.raw[i] = b128::load8_edge(from, p.ncol, a.src_vec);
+      }
     }
-    // Maxima of the piece's rows and columns, as bits; once more over the
-    // finite values alone where the tile has others.
-    bool any = false;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-      uint32_t rmax[8], cmax[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) rmax[i] = cmax[i] = 0;
-      if (pass == 0) {
-        b128::tops(p.raw, rmax, cmax);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float v[8];
-          b128::unpack(p.raw[i], v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t m = __float_as_uint(b128::finite_magnitude(v[j]));
-            rmax[i] = max(rmax[i], m);
-            cmax[j] = max(cmax[j], m);
-          }
-        }
-      }
-      if (a.block_rows == kBlock) {  // one maximum: rows of the piece stand for all
-#pragma unroll
-        for (int i = 1; i < 8; ++i) rmax[0] = max(rmax[0], rmax[i]);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-          rmax[0] = max(rmax[0], __shfl_xor_sync(0xffffffffu, rmax[0], o));
-        if (lane == 0) row_part[wc][wr] = rmax[0];
-      } else {
-        if (a.dst != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // over the 4 lanes of a row, then the 4 warps
-            rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 1));
-            rmax[i] = max(rmax[i], __shfl_xor_sync(0xffffffffu, rmax[i], 2));
-          }
-          if (lc == 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) row_part[wc][row_in + i] = rmax[i];
-          }
-        }
-        if (a.dst_t != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1)
-              cmax[i] = max(cmax[i], __shfl_xor_sync(0xffffffffu, cmax[i], o));
-          if (lr == 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) col_part[wr][col_in + i] = cmax[i];
-          }
-        }
-      }
-      __syncthreads();
-      // thread t: row t of the tile, or column t - 128
-      const int k = threadIdx.x & 127;
-      const bool is_row = threadIdx.x < 128;
-      uint32_t top = 0;
-      if (a.block_rows == kBlock) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, row_part[i & 3][i >> 2]);
-      } else if (is_row && a.dst != nullptr) {
-        top = max(max(row_part[0][k], row_part[1][k]), max(row_part[2][k], row_part[3][k]));
-      } else if (!is_row && a.dst_t != nullptr) {
-        top = max(col_part[0][k], col_part[1][k]);
-      }
-      const uint32_t byte = b128::scale_byte(__uint_as_float(top));
-      (is_row ? row_inv : col_inv)[k] = b128::scale_reciprocal(byte);
-      if (pass == 0) {
-        any = __syncthreads_or(top >= b128::kInfBits);
-        if (any) continue;
-      } else {
-        __syncthreads();
-      }
-      const int tall = a.block_rows == 1 ? 1 : kBlock;  // rows that share a scale
-      const int r = tile_r * kBlock + k, c = blockIdx.x * kBlock + k;
-      if (is_row && a.dst != nullptr && r < a.rows && k % tall == 0)
-        a.scale[(size_t)(r / tall) * a.ld_scale + blockIdx.x] = static_cast<uint8_t>(byte);
-      if (!is_row && a.dst_t != nullptr && c < a.cols && k % tall == 0)
-        a.scale_t[(size_t)(c / tall) * a.ld_scale_t + tile_r] = static_cast<uint8_t>(byte);
-      break;
-    }
-    if (any) store_piece<true>(a, p, row_inv + row_in, col_inv + col_in);
-    else store_piece<false>(a, p, row_inv + row_in, col_inv + col_in);
+    const bool any = tile_scales<true>(a, p, tile_r, row_in, col_in, sh);
+    if (any) tile_scales<false>(a, p, tile_r, row_in, col_in, sh);
+    if (whole && !any) store_piece<true>(a, p, sh.row_inv + row_in, sh.col_inv + col_in);
+    else store_piece<false>(a, p, sh.row_inv + row_in, sh.col_inv + col_in);
     __syncthreads();  // the reciprocals are read before the next tile writes them
   }
 }
