@@ -22,7 +22,7 @@ namespace {
 
 using b128::Raw8;
 
-constexpr int kMaxParts = 1024;  // rows of partial weight gradients in the workspace
+constexpr int kMaxParts = 1024;  // CTAs, each with a row of partial weight gradients
 // Rows in the ring.  Two leave room for two CTAs of a wide row on a SM, which
 // counts for more than depth: the backward pass of 8192 x 8192 bf16 takes 90 us
 // with two, 108 with three or four (one CTA a SM); the norm 81, 80 and 102.
@@ -375,15 +375,18 @@ int launch_rows(void (*kernel)(A), const A &a, int grid, int threads, size_t sme
   return CMB_OK;
 }
 
-// How many CTAs walk over the rows: what fits on the device at once, with 64
-// registers a thread and `smem` bytes a CTA.
+// How many CTAs walk over the rows: at most what fits on the device at once,
+// with 64 registers a thread and `smem` bytes a CTA, in even shares (1000 x
+// 4600 backward: 334 CTAs of 3 rows 14.9 us, 444 of 2 or 3 16.1 us).
 int ctas_for(int rows, int threads, size_t smem) {
   int fit = 1024 / threads;
   const int by_smem = static_cast<int>(220 * 1024 / (smem + 1024));
   if (fit > by_smem) fit = by_smem;
   if (fit > 32) fit = 32;
-  const int most = current_sm_count() * (fit > 0 ? fit : 1);
-  return rows < most ? rows : most;
+  int most = current_sm_count() * (fit > 0 ? fit : 1);
+  if (most > kMaxParts) most = kMaxParts;
+  const int each = (rows + most - 1) / most;
+  return (rows + each - 1) / each;
 }
 
 constexpr size_t kRingMost = 200 * 1024;
@@ -415,7 +418,6 @@ int launch_back(NormBackArgs a, int *grid, cudaStream_t stream) {
   const bool use_ring = a.rows > direct && a.cols % 8 == 0 && a.dy_vec && a.h_vec &&
                         (a.dh == nullptr || a.dh_vec) && ring <= kRingMost;
   *grid = use_ring ? ctas_for(a.rows, threads, ring) : direct;
-  if (*grid > kMaxParts) *grid = kMaxParts;
   if (use_ring) return launch_rows(k_rmsnorm_back<T, W, NV, true>, a, *grid, threads, ring, stream);
   return launch_rows(k_rmsnorm_back<T, W, NV, false>, a, *grid, threads, 0, stream);
 }
