@@ -47,10 +47,6 @@ __device__ __forceinline__ float scale_reciprocal(uint32_t byte) {
 // look at it tells whether a block has anything that is not finite.
 constexpr uint32_t kInfBits = 0x7F800000u;
 
-__device__ __forceinline__ uint32_t magnitude_bits(float x) {
-  return __float_as_uint(x) & 0x7FFFFFFFu;
-}
-
 // Four values to e4m3 (nearest even), the first in the low byte.  The scale
 // keeps finite values within 448, so saturation only ever meets infinities;
 // where a block may hold any (kAny), those become NaN, as NaN does.
@@ -72,6 +68,39 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return q;
 }
 
+// The larger magnitude; NaN wins.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// a * b + c, both halves at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %5};\n\t"
+      "mov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, w; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 // a * s, both halves at once.
 __device__ __forceinline__ float2 mul2(float2 a, float2 s) {
   float2 r;
@@ -87,11 +116,11 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 s) {
 
 // 8 values times `inv` as 8 e4m3 bytes.
 template <bool kAny>
-__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
+__device__ __forceinline__ uint2 e4m3x8(const float2 (&v)[4], float inv) {
   const float2 s = make_float2(inv, inv);
   float2 p[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = mul2(make_float2(v[2 * i], v[2 * i + 1]), s);
+  for (int i = 0; i < 4; ++i) p[i] = mul2(v[i], s);
   return make_uint2(e4m3x4<kAny>(p[0].x, p[0].y, p[1].x, p[1].y),
                     e4m3x4<kAny>(p[2].x, p[2].y, p[3].x, p[3].y));
 }
@@ -223,6 +252,14 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+template <typename T>
+__device__ __forceinline__ void unpack2(const Raw8<T> &r, float2 (&v)[4]) {
+  float u[8];
+  unpack(r, u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = make_float2(u[2 * i], u[2 * i + 1]);
+}
+
 // Rounded (nearest even) to the type of the row.
 __device__ __forceinline__ void pack(const float (&v)[8], Raw8<__nv_bfloat16> &r) {
   r.a = make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]),
@@ -235,6 +272,14 @@ __device__ __forceinline__ void pack(const float (&v)[8], Raw8<float> &r) {
                    __float_as_uint(v[7]));
 }
 
+template <typename T>
+__device__ __forceinline__ Raw8<T> packed(const float2 (&v)[4]) {
+  const float u[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+  Raw8<T> r;
+  pack(u, r);
+  return r;
+}
+
 __device__ __forceinline__ void store8(__nv_bfloat16 *p, const Raw8<__nv_bfloat16> &r) {
   *reinterpret_cast<uint4 *>(p) = r.a;
 }
@@ -243,11 +288,66 @@ __device__ __forceinline__ void store8(float *p, const Raw8<float> &r) {
   reinterpret_cast<uint4 *>(p)[1] = r.b;
 }
 
-// Elements [0, n) of the 8 at p, zeros behind them; whole aligned chunks in
-// one or two 16-byte loads.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8_edge(const T *p, int n, bool aligned) {
-  if (aligned && n >= 8) return load8(p);
+__device__ __forceinline__ void words_of(const Raw8<T> &r, uint32_t (&w)[sizeof(T) * 2]) {
+  w[0] = r.a.x, w[1] = r.a.y, w[2] = r.a.z, w[3] = r.a.w;
+  if constexpr (sizeof(T) == 4) w[4] = r.b.x, w[5] = r.b.y, w[6] = r.b.z, w[7] = r.b.w;
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> from_words(const uint32_t *w) {
+  Raw8<T> r;
+  r.a = make_uint4(w[0], w[1], w[2], w[3]);
+  if constexpr (sizeof(T) == 4) r.b = make_uint4(w[4], w[5], w[6], w[7]);
+  return r;
+}
+
+// out[i] = the 4 bytes at byte `m` (0-15) + 4 i of the words in.
+template <int N>
+__device__ __forceinline__ void from_byte(uint32_t (&in)[N + 4], uint32_t m, uint32_t (&out)[N]) {
+#pragma unroll
+  for (int step = 2; step > 0; step >>= 1)
+#pragma unroll
+    for (int i = 0; i + step < N + 4; ++i) in[i] = (m >> 2) & step ? in[i + step] : in[i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(in[i], in[i + 1], 8 * (m & 3));
+}
+
+// Where a matrix begins and ends.  Chunks of rows at odd addresses are cut out
+// of the aligned 16-byte pieces around them, which has to stay inside.
+struct Bounds {
+  uintptr_t begin, end;
+  template <typename T>
+  static __device__ __forceinline__ Bounds of(const T *p, size_t ld, int rows, int cols) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+    return {b, b + (static_cast<size_t>(rows - 1) * ld + cols) * sizeof(T)};
+  }
+};
+
+// Elements [0, n) of the 8 at p, zeros behind them.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_any(const T *p, int n, const Bounds &in) {
+  constexpr int N = sizeof(T) * 2;  // words
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), piece = at & ~uintptr_t(15);
+  uint32_t w[N];
+  if (n <= 0) return Raw8<T>{};
+  if (at == piece && n >= 8) return load8(p);
+  if (piece >= in.begin && piece + 4 * N + 16 <= in.end) {
+    uint32_t c[N + 4];
+#pragma unroll
+    for (int i = 0; i < N / 4 + 1; ++i) {
+      const uint4 v = reinterpret_cast<const uint4 *>(piece)[i];
+      c[4 * i] = v.x, c[4 * i + 1] = v.y, c[4 * i + 2] = v.z, c[4 * i + 3] = v.w;
+    }
+    from_byte<N>(c, static_cast<uint32_t>(at - piece), w);
+    if (n < 8) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int left = n * static_cast<int>(sizeof(T)) - 4 * i;  // bytes of this word
+        if (left < 4) w[i] = left > 0 ? w[i] & ((1u << (8 * left)) - 1) : 0u;
+      }
+    }
+    return from_words<T>(w);
+  }
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.0f;
@@ -257,16 +357,46 @@ __device__ __forceinline__ Raw8<T> load8_edge(const T *p, int n, bool aligned) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store8_edge(T *p, const Raw8<T> &r, int n, bool aligned) {
-  if (aligned && n >= 8) {
-    store8(p, r);
-    return;
-  }
+__device__ __forceinline__ void store_elements(T *p, const Raw8<T> &r, int from, int to) {
   float v[8];
   unpack(r, v);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = from_float<T>(v[i]);
+    if (i >= from && i < to) p[i] = from_float<T>(v[i]);
+}
+
+// Writes elements [0, n) of the 8 to p.  The whole warp, whose lanes have
+// consecutive chunks: where they do not start on 16 bytes, a lane takes the end
+// of the chunk before its own from its neighbour and writes the aligned pieces.
+template <typename T>
+__device__ __forceinline__ void store8_any(T *p, const Raw8<T> &r, int n) {
+  constexpr int N = sizeof(T) * 2;  // words
+  const uint32_t m = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15);
+  if (m == 0) {  // the same in all lanes
+    if (n >= 8) store8(p, r);
+    else store_elements(p, r, 0, n);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  uint32_t w[N], c[N + 4], out[N];
+  words_of(r, w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = __shfl_up_sync(0xffffffffu, w[N - 4 + i], 1);
+#pragma unroll
+  for (int i = 0; i < N; ++i) c[4 + i] = w[i];
+  const uint32_t fulls = __ballot_sync(0xffffffffu, n >= 8);
+  from_byte<N>(c, 16 - m, out);
+  if (n < 8) {
+    store_elements(p, r, 0, n);
+    return;
+  }
+  const bool joins = lane > 0 && (fulls >> (lane - 1)) & 1, next = lane < 31 && (fulls >> (lane + 1)) & 1;
+  uint4 *piece = reinterpret_cast<uint4 *>(reinterpret_cast<uintptr_t>(p) - m);
+  const int head = static_cast<int>((16 - m) / sizeof(T)), tail = 8 - static_cast<int>(m / sizeof(T));
+  if (joins) piece[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  else store_elements(p, r, 0, head);
+  if constexpr (N == 8) piece[1] = make_uint4(out[4], out[5], out[6], out[7]);
+  if (!next) store_elements(p, r, tail, 8);
 }
 
 // 8 bytes, or the first n of them; the odd case out of the way of the other.

@@ -37,8 +37,8 @@ __device__ __forceinline__ uint2 row_bytes(const Raw8<__nv_bfloat16> &r, float i
 }
 template <bool kAny>
 __device__ __forceinline__ uint2 row_bytes(const Raw8<float> &r, float inv) {
-  float v[8];
-  b128::unpack(r, v);
+  float2 v[4];
+  b128::unpack2(r, v);
   return b128::e4m3x8<kAny>(v, inv);
 }
 
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const QuantArgs a) {
   const long long total = (long long)a.rows * groups;
   dev::grid_dep_wait();
   dev::grid_dep_launch();
+  const b128::Bounds in = b128::Bounds::of(src, a.ld_src, a.rows, a.cols);
   // warp-uniform bound: both halves of a warp take part in the shuffles
   const long long me = (long long)blockIdx.x * (blockDim.x / 16) + threadIdx.x / 16;
   for (long long base = me & ~1LL; base < total; base += half_warps * kUnroll) {
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const QuantArgs a) {
       const int col = group[u] * kBlock + lane16 * 8;
       raw[u] = {};
       if (at[u] < total && col < a.cols)
-        raw[u] = b128::load8_edge(src + (size_t)row[u] * a.ld_src + col, a.cols - col, a.src_vec);
+        raw[u] = b128::load8_any(src + (size_t)row[u] * a.ld_src + col, a.cols - col, in);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -134,7 +135,8 @@ __device__ __forceinline__ void column_bytes(const Raw8<float> (&raw)[8], int k,
       const int at = 2 * (k & 1) + d;
       v[i] = __uint_as_float(at == 0 ? r.x : at == 1 ? r.y : at == 2 ? r.z : r.w);
     }
-    q[d] = b128::e4m3x8<kAny>(v, d == 0 ? inv0 : inv1);
+    const float2 u[4] = {{v[0], v[1]}, {v[2], v[3]}, {v[4], v[5]}, {v[6], v[7]}};
+    q[d] = b128::e4m3x8<kAny>(u, d == 0 ? inv0 : inv1);
   }
 }
 
@@ -270,8 +272,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize_tile(c
   Piece<T> p;
   p.col = blockIdx.x * kBlock + col_in;
   p.ncol = min(8, a.cols - p.col);
-  const bool wide = (blockIdx.x + 1) * kBlock <= a.cols && a.src_vec &&
-                    (a.dst == nullptr || a.dst_vec) && (a.dst_t == nullptr || a.dst_t_vec);
+  // a tile that is all there is stored without a look at its edges; where its
+  // rows start is the loads' business
+  const bool wide = (blockIdx.x + 1) * kBlock <= a.cols && (a.dst == nullptr || a.dst_vec) &&
+                    (a.dst_t == nullptr || a.dst_t_vec);
+  const b128::Bounds in = b128::Bounds::of(src, a.ld_src, a.rows, a.cols);
   dev::grid_dep_wait();
   dev::grid_dep_launch();
 
@@ -280,14 +285,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize_tile(c
     p.nrow = min(8, a.rows - p.row);
     const T *from = src + (size_t)p.row * a.ld_src + p.col;
     const bool whole = wide && (tile_r + 1) * kBlock <= a.rows;
-    if (whole) {
+    if (whole && a.src_vec) {
 #pragma unroll
       for (int i = 0; i < 8; ++i, from += a.ld_src) p.raw[i] = b128::load8(from);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i, from += a.ld_src) {
         p.raw[i] = {};
-        if (i < p.nrow && p.ncol > 0) p.raw[i] = b128::load8_edge(from, p.ncol, a.src_vec);
+        if (i < p.nrow) p.raw[i] = b128::load8_any(from, p.ncol, in);
       }
     }
     const bool any = tile_scales<true>(a, p, tile_r, row_in, col_in, sh);

@@ -8,18 +8,23 @@
 // its backward pass and every later reader then see the same h.  Sums and
 // statistics are fp32, in a fixed order.
 //
-// A CTA works on a whole row.  Two ways to read rows (template kRing):
-//   ring    rows that start and end on 16 bytes, several rows a CTA: a thread
-//           keeps the next rows on their way into shared memory with bulk
-//           copies, so loads never wait for a row's reduction.
-//   direct  everything else, and calls with no more rows than CTAs, whose
-//           latency is one load.
+// A CTA of blockDim.x x blockDim.y threads works on blockDim.y rows at a time;
+// thread x holds the chunks of 8 columns x, x + blockDim.x, ...: a warp stays
+// within a row, and 16 neighbouring threads hold a block of 128.  Three ways to
+// read and write rows (Way):
+//   kRing  whole chunks that start on 16 bytes, several rows a CTA: a thread
+//          keeps the next rows on their way into shared memory with bulk
+//          copies, so loads never wait for a row's reduction.
+//   kFew   the same with no more rows than the device has room for at once:
+//          straight from global memory, since latency is one load.
+//   kAny   every other width, pitch and alignment.
 #include "block128.cuh"
 #include "cmb_host.h"
 
 namespace cmb {
 namespace {
 
+using b128::Bounds;
 using b128::Raw8;
 
 constexpr int kMaxParts = 1024;  // CTAs, each with a row of partial weight gradients
@@ -28,58 +33,117 @@ constexpr int kMaxParts = 1024;  // CTAs, each with a row of partial weight grad
 // with two, 108 with three or four (one CTA a SM); the norm 81, 80 and 102.
 constexpr int kStages = 2;
 
-// Sum over the CTA, the same value in every thread.  `part` holds one float
-// for each warp; two calls in a row use different ones.
-__device__ __forceinline__ float cta_sum(float v, float *part) {
+enum Way { kRing, kFew, kAny };
+
+// Sum over the threads of a row, the same value in each.  `part` holds one
+// float for each warp; two calls in a row use different ones.
+__device__ __forceinline__ float row_sum(float v, float *part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) part[warp] = v;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  part += threadIdx.y * warps;
+  if (lane == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
-  const int warps = blockDim.x >> 5;
   v = lane < warps ? part[lane] : 0.0f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Rows of up to three matrices on their way through shared memory: row i of
-// a CTA (its rows are blockIdx.x, + gridDim.x, ...) in stage i % kStages.
+// Rows of up to three matrices on their way through shared memory.  A CTA's
+// turn i is over rows (blockIdx.x + i * gridDim.x) * blockDim.y and on, in stage
+// i % kStages.
 struct Ring {
   const uint8_t *src[3];
   size_t pitch[3];
-  int n;          // matrices
+  int n;           // matrices
   uint32_t bytes;  // of a row of one of them
   uint8_t *mem;
   uint64_t *full;
 
   __device__ __forceinline__ void load(int i, int rows) const {
-    const long long row = blockIdx.x + static_cast<long long>(i) * gridDim.x;
-    if (row >= rows) return;
+    const long long first = (blockIdx.x + static_cast<long long>(i) * gridDim.x) * blockDim.y;
+    if (first >= rows) return;
+    const int high = static_cast<int>(min(static_cast<long long>(blockDim.y), rows - first));
     const int s = i % kStages;
     const uint32_t bar = dev::smem_addr(full + s);
-    dev::mbar_arrive_expect_tx(bar, bytes * n);
-    for (int k = 0; k < n; ++k)
-      dev::bulk_load(dev::smem_addr(mem + (size_t)(s * n + k) * bytes), src[k] + row * pitch[k],
-                     bytes, bar);
+    dev::mbar_arrive_expect_tx(bar, bytes * n * high);
+    for (int y = 0; y < high; ++y)
+      for (int k = 0; k < n; ++k)
+        dev::bulk_load(dev::smem_addr(at(s, y, k)), src[k] + (first + y) * pitch[k], bytes, bar);
   }
   __device__ __forceinline__ void start(int rows) const {
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && threadIdx.y == 0) {
       for (int s = 0; s < kStages; ++s) dev::mbar_init(dev::smem_addr(full + s), 1);
       dev::fence_mbar_init();
     }
     __syncthreads();
-    if (threadIdx.x == 0)
+    if (threadIdx.x == 0 && threadIdx.y == 0)
       for (int s = 0; s < kStages; ++s) load(s, rows);
   }
-  // Waits for row i; a bulk copy of this GPU's own memory ends, or the launch
+  // Waits for turn i; a bulk copy of this GPU's own memory ends, or the launch
   // has failed as a whole.
   __device__ __forceinline__ void wait(int i) const {
     dev::mbar_wait_bounded(dev::smem_addr(full + i % kStages), (i / kStages) & 1);
   }
+  __device__ __forceinline__ uint8_t *at(int s, int y, int k) const {
+    return mem + static_cast<size_t>((s * static_cast<int>(blockDim.y) + y) * n + k) * bytes;
+  }
   template <typename T>
   __device__ __forceinline__ const T *row(int i, int k) const {
-    return reinterpret_cast<const T *>(mem + (size_t)(i % kStages * n + k) * bytes);
+    return reinterpret_cast<const T *>(at(i % kStages, threadIdx.y, k));
+  }
+};
+
+// 8 columns of a row, from the ring or from where the row lies.
+template <typename T, int kWay>
+__device__ __forceinline__ Raw8<T> load_chunk(const Ring &ring, int turn, int k, const void *p,
+                                              size_t ld, int row, int col, int n,
+                                              const Bounds &in) {
+  if (n <= 0) return {};
+  if constexpr (kWay == kRing) return b128::load8(ring.row<T>(turn, k) + col);
+  const T *at = static_cast<const T *>(p) + static_cast<size_t>(row) * ld + col;
+  if constexpr (kWay == kFew) return b128::load8(at);
+  else return b128::load8_any(at, n, in);
+}
+
+// The whole warp (see b128::store8_any).
+template <typename T, int kWay>
+__device__ __forceinline__ void store_chunk(void *p, size_t ld, int row, int col, int n,
+                                            const Raw8<T> &r) {
+  T *at = static_cast<T *>(p) + static_cast<size_t>(row) * ld + col;
+  if constexpr (kWay == kAny) {
+    b128::store8_any(at, r, n);
+  } else {
+    if (n > 0) b128::store8(at, r);
+  }
+}
+
+// A thread's chunks of the weights: kept in registers, or, where a row has
+// more than two chunks a thread, read again for each row.
+template <typename W, int NV>
+struct Weight {
+  const W *p;
+  Bounds in;
+  int cols;
+  Raw8<W> kept[NV <= 2 ? NV : 1];
+
+  __device__ __forceinline__ Weight(const void *weight, int cols)
+      : p(static_cast<const W *>(weight)),
+        in(Bounds::of(static_cast<const W *>(weight), 0, 1, cols)),
+        cols(cols) {
+    if constexpr (NV <= 2) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) kept[i] = load(i);
+    }
+  }
+  __device__ __forceinline__ Raw8<W> load(int i) const {
+    const int col = (i * blockDim.x + threadIdx.x) * 8;
+    return b128::load8_any(p + col, cols - col, in);
+  }
+  __device__ __forceinline__ Raw8<W> chunk(int i) const {
+    if constexpr (NV <= 2) return kept[i];
+    else return load(i);
   }
 };
 
@@ -91,142 +155,111 @@ struct NormArgs {
   size_t ld_x, ld_r, ld_h, ld_y, ld_q, ld_scale;
   float eps;
   int rows, cols;
-  bool x_vec, r_vec, w_vec, h_vec, y_vec, q_vec;
+  bool q_vec;  // 8-byte stores of q
 };
 
-// The e4m3 values and scales of 8 columns of a row; 16 neighbouring threads
-// have a block of 128.
-__device__ __forceinline__ void store_quantized(const NormArgs &a, int row, int col,
-                                                const float (&y)[8]) {
-  const int n = a.cols - col;
-  uint32_t top = 0;
+// The e4m3 values and scales of 8 columns of a row; the whole warp.
+__device__ __forceinline__ void store_quantized(const NormArgs &a, int row, int col, int n,
+                                                const float2 (&y)[4]) {
+  float top = b128::max_magnitude(y[0].x, y[0].y);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, b128::magnitude_bits(y[j]));
+  for (int j = 1; j < 4; ++j)
+    top = b128::max_magnitude(top, b128::max_magnitude(y[j].x, y[j].y));
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const bool any = __any_sync(0xffffffffu, top >= b128::kInfBits);
+  for (int o = 1; o < 16; o <<= 1)
+    top = b128::max_magnitude(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool any = __any_sync(0xffffffffu, !(top <= b128::kMaxFinite));
   if (any) {  // the scale is that of the finite values
-    float m = 0.0f;
+    top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, b128::finite_magnitude(y[j]));
+    for (int j = 0; j < 4; ++j)
+      top = fmaxf(top, fmaxf(b128::finite_magnitude(y[j].x), b128::finite_magnitude(y[j].y)));
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    top = __float_as_uint(m);
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
-  const uint32_t byte = b128::scale_byte(__uint_as_float(top));
+  const uint32_t byte = b128::scale_byte(top);
   const float inv = b128::scale_reciprocal(byte);
   if (n > 0) {
-    b128::store_bytes(a.q + (size_t)row * a.ld_q + col,
+    b128::store_bytes(a.q + static_cast<size_t>(row) * a.ld_q + col,
                       any ? b128::e4m3x8<true>(y, inv) : b128::e4m3x8<false>(y, inv), n, a.q_vec);
     if ((threadIdx.x & 15) == 0)
-      a.scale[(size_t)row * a.ld_scale + col / b128::kBlock] = static_cast<uint8_t>(byte);
+      a.scale[static_cast<size_t>(row) * a.ld_scale + col / b128::kBlock] =
+          static_cast<uint8_t>(byte);
   }
 }
 
-// A thread's chunks of the weights: kept in registers, or, where a row has
-// more than two chunks a thread, read again for each row.
-template <typename W, int NV>
-struct Weight {
-  const W *p;
-  bool vec;
-  Raw8<W> kept[NV <= 2 ? NV : 1];
-
-  __device__ __forceinline__ Weight(const void *weight, bool aligned, int cols)
-      : p(static_cast<const W *>(weight)), vec(aligned) {
-    if constexpr (NV <= 2) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = (i * blockDim.x + threadIdx.x) * 8;
-        kept[i] = load(col, cols - col);
-      }
-    }
-  }
-  __device__ __forceinline__ Raw8<W> load(int col, int n) const {
-    return n > 0 ? b128::load8_edge(p + col, n, vec) : Raw8<W>{};
-  }
-  __device__ __forceinline__ Raw8<W> chunk(int i, int col, int n) const {
-    if constexpr (NV <= 2) return kept[i];
-    else return load(col, n);
-  }
-};
-
-// Thread t holds the chunks of 8 columns t, t + blockDim, ...: 16
-// neighbouring threads hold a block of 128.
-template <typename T, typename W, int NV, bool kRing>
+template <typename T, typename W, int NV, int kWay>
 __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
   __shared__ float part[2][32];
   __shared__ __align__(8) uint64_t full[kStages];
   extern __shared__ __align__(16) uint8_t rows_mem[];
-  const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.residual);
   dev::grid_dep_wait();
   dev::grid_dep_launch();
-  Ring ring;
-  if constexpr (kRing) {
+  Ring ring = {};
+  if constexpr (kWay == kRing) {
     ring = {{static_cast<const uint8_t *>(a.x), static_cast<const uint8_t *>(a.residual), nullptr},
             {a.ld_x * sizeof(T), a.ld_r * sizeof(T), 0},
-            res != nullptr ? 2 : 1,
+            a.residual != nullptr ? 2 : 1,
             static_cast<uint32_t>(a.cols * sizeof(T)),
             rows_mem,
             full};
     ring.start(a.rows);
   }
-  const Weight<W, NV> weight(a.weight, a.w_vec, a.cols);
-  int it = 0;
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
-    Raw8<T> h[NV];  // as it is stored
-    float sq = 0.0f;
-    if constexpr (kRing) ring.wait(it);
+  Bounds in_x{}, in_r{};
+  if constexpr (kWay == kAny) {
+    in_x = Bounds::of(static_cast<const T *>(a.x), a.ld_x, a.rows, a.cols);
+    in_r = Bounds::of(static_cast<const T *>(a.residual), a.ld_r, a.rows, a.cols);
+  }
+  const Weight<W, NV> weight(a.weight, a.cols);
+  int turn = 0;
+  for (int first = blockIdx.x * blockDim.y; first < a.rows;
+       first += gridDim.x * blockDim.y, ++turn) {
+    const int row = first + threadIdx.y;
+    const bool here = row < a.rows;  // the same in a warp
+    Raw8<T> h[NV];                   // as it is stored
+    float2 sq = make_float2(0.0f, 0.0f);
+    if constexpr (kWay == kRing) ring.wait(turn);
+    if (here) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      Raw8<T> raw{}, add{};
-      if (n > 0) {
-        if constexpr (kRing) {
-          raw = b128::load8(ring.row<T>(it, 0) + col);
-          if (res != nullptr) add = b128::load8(ring.row<T>(it, 1) + col);
-        } else {
-          raw = b128::load8_edge(x + (size_t)row * a.ld_x + col, n, a.x_vec);
-          if (res != nullptr) add = b128::load8_edge(res + (size_t)row * a.ld_r + col, n, a.r_vec);
-        }
-        if (res != nullptr) {
-          float v[8], u[8];
-          b128::unpack(raw, v);
-          b128::unpack(add, u);
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
+        h[i] = load_chunk<T, kWay>(ring, turn, 0, a.x, a.ld_x, row, col, n, in_x);
+        float2 v[4];
+        b128::unpack2(h[i], v);
+        if (a.residual != nullptr) {
+          float2 u[4];
+          b128::unpack2(
+              load_chunk<T, kWay>(ring, turn, 1, a.residual, a.ld_r, row, col, n, in_r), u);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] += u[j];
-          b128::pack(v, raw);
-          b128::store8_edge(static_cast<T *>(a.h) + (size_t)row * a.ld_h + col, raw, n, a.h_vec);
+          for (int j = 0; j < 4; ++j) v[j] = b128::add2(v[j], u[j]);
+          h[i] = b128::packed<T>(v);
+          store_chunk<T, kWay>(a.h, a.ld_h, row, col, n, h[i]);
+          b128::unpack2(h[i], v);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sq = b128::fma2(v[j], v[j], sq);
       }
-      h[i] = raw;
-      float v[8];
-      b128::unpack(raw, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sq = fmaf(v[j], v[j], sq);
     }
-    sq = cta_sum(sq, part[it & 1]);
-    if constexpr (kRing)
-      if (threadIdx.x == 0) ring.load(it + kStages, a.rows);  // every thread has its chunks
-    const float rstd = 1.0f / sqrtf(sq / static_cast<float>(a.cols) + a.eps);
+    const float sum = row_sum(sq.x + sq.y, part[turn & 1]);
+    if constexpr (kWay == kRing)
+      if (threadIdx.x == 0 && threadIdx.y == 0)
+        ring.load(turn + kStages, a.rows);  // every thread has its chunks
+    if (!here) continue;
+    const float rstd = 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps);
     if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      float y[8], wv[8];
-      b128::unpack(h[i], y);
-      b128::unpack(weight.chunk(i, col, n), wv);
+      float2 y[4], w[4];
+      b128::unpack2(h[i], y);
+      b128::unpack2(weight.chunk(i), w);
+      // behind the row's end h is 0 and y too, or NaN where rstd is not finite,
+      // which a block's scale passes over
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] = y[j] * rstd * wv[j];
-        // behind the row's end: not 0 * inf, which would be NaN
-        if (j >= n) y[j] = 0.0f;
-      }
-      if (a.y != nullptr && n > 0) {
-        Raw8<T> out;
-        b128::pack(y, out);
-        b128::store8_edge(static_cast<T *>(a.y) + (size_t)row * a.ld_y + col, out, n, a.y_vec);
-      }
-      if (a.q != nullptr) store_quantized(a, row, col, y);
+      for (int j = 0; j < 4; ++j)
+        y[j] = b128::mul2(b128::mul2(y[j], make_float2(rstd, rstd)), w[j]);
+      if (a.y != nullptr) store_chunk<T, kWay>(a.y, a.ld_y, row, col, n, b128::packed<T>(y));
+      if (a.q != nullptr) store_quantized(a, row, col, n, y);
     }
   }
 }
@@ -238,21 +271,20 @@ struct NormBackArgs {
   float *parts;  // gridDim.x rows of cols partial weight gradients, or NULL
   size_t ld_dy, ld_h, ld_dh, ld_dx, ld_parts;
   int rows, cols;
-  bool dy_vec, h_vec, dh_vec, w_vec, dx_vec;
 };
 
 // Both passes over a row read it from where it lies, the ring's shared memory
-// or (direct) global memory, so a thread holds no more of it than a chunk; the
-// weight gradient of its columns stays in registers from row to row.
-template <typename T, typename W, int NV, bool kRing>
+// or global memory, so a thread holds no more of it than a chunk; the weight
+// gradient of its columns stays in registers from row to row.
+template <typename T, typename W, int NV, int kWay>
 __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) {
   __shared__ float part[2][32];
   __shared__ __align__(8) uint64_t full[kStages];
   extern __shared__ __align__(16) uint8_t rows_mem[];
   dev::grid_dep_wait();
   dev::grid_dep_launch();
-  Ring ring;
-  if constexpr (kRing) {
+  Ring ring = {};
+  if constexpr (kWay == kRing) {
     ring = {{static_cast<const uint8_t *>(a.dy), static_cast<const uint8_t *>(a.h),
              static_cast<const uint8_t *>(a.dh)},
             {a.ld_dy * sizeof(T), a.ld_h * sizeof(T), a.ld_dh * sizeof(T)},
@@ -262,62 +294,93 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
             full};
     ring.start(a.rows);
   }
-  const Weight<W, NV> weight(a.weight, a.w_vec, a.cols);
-  float dw[NV][8] = {};
-  int it = 0;
-  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, ++it) {
-    const auto load = [&](int k, const void *p, size_t ld, int col, int n, bool vec) {
-      if constexpr (kRing) return b128::load8(ring.row<T>(it, k) + col);
-      else return b128::load8_edge(static_cast<const T *>(p) + (size_t)row * ld + col, n, vec);
-    };
-    const float rstd = a.rstd[row];
-    float along = 0.0f;
-    if constexpr (kRing) ring.wait(it);
+  Bounds in_dy{}, in_h{}, in_dh{};
+  if constexpr (kWay == kAny) {
+    in_dy = Bounds::of(static_cast<const T *>(a.dy), a.ld_dy, a.rows, a.cols);
+    in_h = Bounds::of(static_cast<const T *>(a.h), a.ld_h, a.rows, a.cols);
+    in_dh = Bounds::of(static_cast<const T *>(a.dh), a.ld_dh, a.rows, a.cols);
+  }
+  const Weight<W, NV> weight(a.weight, a.cols);
+  float2 dw[NV][4] = {};
+  int turn = 0;
+  for (int first = blockIdx.x * blockDim.y; first < a.rows;
+       first += gridDim.x * blockDim.y, ++turn) {
+    const int row = first + threadIdx.y;
+    const bool here = row < a.rows;  // the same in a warp
+    const float rstd = here ? a.rstd[row] : 0.0f;
+    const float2 rstd2 = make_float2(rstd, rstd);
+    float2 along = make_float2(0.0f, 0.0f);
+    if constexpr (kWay == kRing) ring.wait(turn);
+    if (here) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      if (n <= 0) continue;
-      float g[8], u[8], wv[8];
-      b128::unpack(load(0, a.dy, a.ld_dy, col, n, a.dy_vec), g);
-      b128::unpack(load(1, a.h, a.ld_h, col, n, a.h_vec), u);
-      b128::unpack(weight.chunk(i, col, n), wv);
+      for (int i = 0; i < NV; ++i) {
+        const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
+        float2 g[4], u[4], w[4];
+        b128::unpack2(load_chunk<T, kWay>(ring, turn, 0, a.dy, a.ld_dy, row, col, n, in_dy), g);
+        b128::unpack2(load_chunk<T, kWay>(ring, turn, 1, a.h, a.ld_h, row, col, n, in_h), u);
+        b128::unpack2(weight.chunk(i), w);
+        if (n > 0) {  // behind the row's end 0 * rstd may be NaN
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // behind the row's end: not 0 * inf, which would be NaN
-        const float unit = j < n ? u[j] * rstd : 0.0f;
-        dw[i][j] = fmaf(g[j], unit, dw[i][j]);
-        along = fmaf(g[j] * wv[j], unit, along);
+          for (int j = 0; j < 4; ++j) {
+            u[j] = b128::mul2(u[j], rstd2);
+            if (kWay == kAny && n < 8) {
+              if (2 * j >= n) u[j].x = 0.0f;
+              if (2 * j + 1 >= n) u[j].y = 0.0f;
+            }
+            dw[i][j] = b128::fma2(g[j], u[j], dw[i][j]);
+            along = b128::fma2(b128::mul2(g[j], w[j]), u[j], along);
+          }
+        }
       }
     }
-    const float mean = cta_sum(along, part[it & 1]) / static_cast<float>(a.cols);
-    // every thread is past the last row: its place takes another
-    if constexpr (kRing)
-      if (threadIdx.x == 0 && it > 0) ring.load(it - 1 + kStages, a.rows);
+    const float mean = row_sum(along.x + along.y, part[turn & 1]) / static_cast<float>(a.cols);
+    // every thread is past the last turn: its place takes another
+    if constexpr (kWay == kRing)
+      if (threadIdx.x == 0 && threadIdx.y == 0 && turn > 0) ring.load(turn - 1 + kStages, a.rows);
+    if (!here) continue;
+    const float2 minus = make_float2(-rstd * mean, -rstd * mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      if (n <= 0) continue;
-      float g[8], u[8], wv[8], past[8] = {};
-      b128::unpack(load(0, a.dy, a.ld_dy, col, n, a.dy_vec), g);
-      b128::unpack(load(1, a.h, a.ld_h, col, n, a.h_vec), u);
-      if (a.dh != nullptr) b128::unpack(load(2, a.dh, a.ld_dh, col, n, a.dh_vec), past);
-      b128::unpack(weight.chunk(i, col, n), wv);
+      float2 g[4], u[4], w[4], past[4] = {};
+      b128::unpack2(load_chunk<T, kWay>(ring, turn, 0, a.dy, a.ld_dy, row, col, n, in_dy), g);
+      b128::unpack2(load_chunk<T, kWay>(ring, turn, 1, a.h, a.ld_h, row, col, n, in_h), u);
+      if (a.dh != nullptr)
+        b128::unpack2(load_chunk<T, kWay>(ring, turn, 2, a.dh, a.ld_dh, row, col, n, in_dh), past);
+      b128::unpack2(weight.chunk(i), w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        g[j] = fmaf(rstd, g[j] * wv[j] - u[j] * rstd * mean, past[j]);
-      Raw8<T> out;
-      b128::pack(g, out);
-      b128::store8_edge(static_cast<T *>(a.dx) + (size_t)row * a.ld_dx + col, out, n, a.dx_vec);
+      for (int j = 0; j < 4; ++j)
+        g[j] = b128::fma2(rstd2, b128::fma2(u[j], minus, b128::mul2(g[j], w[j])), past[j]);
+      store_chunk<T, kWay>(a.dx, a.ld_dx, row, col, n, b128::packed<T>(g));
     }
   }
-  if (a.parts != nullptr) {
+  if (a.parts == nullptr) return;
+  // The CTA's rows of threads add theirs up, in order, where the ring was (or
+  // in memory of their own), and the first writes the sum.
+  float4 *sums = reinterpret_cast<float4 *>(rows_mem);
+  for (int y = blockDim.y - 1; y >= 0; --y) {
+    if (y != static_cast<int>(blockDim.y) - 1 || kWay == kRing) __syncthreads();
+    if (static_cast<int>(threadIdx.y) != y) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = (i * blockDim.x + threadIdx.x) * 8;
-      Raw8<float> r;
-      b128::pack(dw[i], r);
-      // the workspace's rows are padded to whole chunks
-      if (col < a.cols) b128::store8(a.parts + (size_t)blockIdx.x * a.ld_parts + col, r);
+      const int chunk = i * blockDim.x + threadIdx.x;
+      float4 v[2] = {{dw[i][0].x, dw[i][0].y, dw[i][1].x, dw[i][1].y},
+                     {dw[i][2].x, dw[i][2].y, dw[i][3].x, dw[i][3].y}};
+      if (chunk * 8 >= a.cols) continue;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float4 *at = sums + 2 * chunk + k;
+        if (y != static_cast<int>(blockDim.y) - 1) {
+          const float4 o = *at;
+          v[k] = make_float4(v[k].x + o.x, v[k].y + o.y, v[k].z + o.z, v[k].w + o.w);
+        }
+        // the workspace's rows are padded to whole chunks
+        if (y == 0)
+          reinterpret_cast<float4 *>(a.parts + static_cast<size_t>(blockIdx.x) * a.ld_parts)
+              [2 * chunk + k] = v[k];
+        else
+          *at = v[k];
+      }
     }
   }
 }
@@ -333,7 +396,7 @@ __global__ void __launch_bounds__(1024) k_sum_parts(const float *__restrict__ pa
   float s = 0.0f;
   if (c < cols) {
 #pragma unroll 8
-    for (int r = threadIdx.y; r < n; r += 32) s += parts[(size_t)r * ld + c];
+    for (int r = threadIdx.y; r < n; r += 32) s += parts[static_cast<size_t>(r) * ld + c];
   }
   sums[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
@@ -344,27 +407,52 @@ __global__ void __launch_bounds__(1024) k_sum_parts(const float *__restrict__ pa
   if (threadIdx.x == 0 && at < cols) out[at] = s;
 }
 
-size_t parts_pitch(int cols) { return ((size_t)cols + 63) / 64 * 64; }
+size_t parts_pitch(int cols) { return (static_cast<size_t>(cols) + 63) / 64 * 64; }
 
-// Chunks of 8 columns a thread, and threads (at most 1024) that hold a row.
-int chunks_for(int cols) { return cols <= 4096 ? 1 : cols <= 16384 ? 2 : 4; }
+// Chunks of 8 columns a thread.  Two up to a width of 16384: a row then takes
+// half the threads, and twice the rows are under way on a SM.
+int chunks_for(int cols) { return cols <= 1024 ? 1 : cols <= 16384 ? 2 : 4; }
 
-int threads_for(int cols, int nv) {
-  const int chunks = (cols + 7) / 8;
-  const int t = (chunks + nv - 1) / nv;
-  return (t + 31) / 32 * 32;
+// CTAs of x * y threads on y rows at a time.
+struct Shape {
+  int x, y, grid;
+  size_t smem;
+};
+
+// `row_bytes`: of a row in the ring, 0 without one.
+Shape shape_for(int rows, int cols, int nv, size_t row_bytes, bool sums) {
+  Shape s;
+  s.x = ((cols + 7) / 8 + nv - 1) / nv;
+  s.x = (s.x + 31) / 32 * 32;
+  // narrow rows: several at a time, as long as every SM has some
+  s.y = 256 / s.x;
+  while (s.y > 1 && rows < s.y * current_sm_count()) s.y /= 2;
+  if (s.y < 1) s.y = 1;
+  s.smem = kStages * row_bytes * s.y;
+  if (sums && s.y > 1 && s.smem < parts_pitch(cols) * sizeof(float))
+    s.smem = parts_pitch(cols) * sizeof(float);
+  // what fits on the device at once, with 64 registers a thread, in even shares
+  // (1000 x 4600 backward: 334 CTAs of 3 rows 14.9 us, 444 of 2 or 3 16.1 us)
+  int fit = 1024 / (s.x * s.y);
+  const int by_smem = static_cast<int>(220 * 1024 / (s.smem + 1024));
+  if (fit > by_smem) fit = by_smem;
+  int most = current_sm_count() * (fit > 0 ? fit : 1);
+  if (most > kMaxParts) most = kMaxParts;
+  const int turns = (rows + s.y - 1) / s.y, each = (turns + most - 1) / most;
+  s.grid = (turns + each - 1) / each;
+  return s;
 }
 
+constexpr size_t kRingMost = 200 * 1024;
+
 template <typename A>
-int launch_rows(void (*kernel)(A), const A &a, int grid, int threads, size_t smem,
-                cudaStream_t stream) {
-  if (smem > 48 * 1024)
-    CMB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(smem)));
+int launch_rows(void (*kernel)(A), const A &a, const Shape &s, cudaStream_t stream) {
+  CMB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(s.smem)));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(s.grid);
+  cfg.blockDim = dim3(s.x, s.y);
+  cfg.dynamicSmemBytes = s.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -375,59 +463,46 @@ int launch_rows(void (*kernel)(A), const A &a, int grid, int threads, size_t sme
   return CMB_OK;
 }
 
-// How many CTAs walk over the rows: at most what fits on the device at once,
-// with 64 registers a thread and `smem` bytes a CTA, in even shares (1000 x
-// 4600 backward: 334 CTAs of 3 rows 14.9 us, 444 of 2 or 3 16.1 us).
-int ctas_for(int rows, int threads, size_t smem) {
-  int fit = 1024 / threads;
-  const int by_smem = static_cast<int>(220 * 1024 / (smem + 1024));
-  if (fit > by_smem) fit = by_smem;
-  if (fit > 32) fit = 32;
-  int most = current_sm_count() * (fit > 0 ? fit : 1);
-  if (most > kMaxParts) most = kMaxParts;
-  const int each = (rows + most - 1) / most;
-  return (rows + each - 1) / each;
-}
-
-constexpr size_t kRingMost = 200 * 1024;
-
+// `plain`: every row of every matrix starts on 16 bytes, and cols % 8 == 0.
 template <typename T, typename W, int NV>
-int launch_norm(const NormArgs &a, cudaStream_t stream) {
-  const int threads = threads_for(a.cols, NV), direct = ctas_for(a.rows, threads, 0);
-  const size_t ring = (size_t)kStages * a.cols * sizeof(T) * (a.residual != nullptr ? 2 : 1);
-  if (a.rows > direct && a.cols % 8 == 0 && a.x_vec && (a.residual == nullptr || a.r_vec) &&
-      ring <= kRingMost)
-    return launch_rows(k_rmsnorm<T, W, NV, true>, a, ctas_for(a.rows, threads, ring), threads,
-                       ring, stream);
-  return launch_rows(k_rmsnorm<T, W, NV, false>, a, direct, threads, 0, stream);
+int launch_norm(const NormArgs &a, bool plain, cudaStream_t stream) {
+  Shape s = shape_for(a.rows, a.cols, NV, 0, false);
+  if (!plain) return launch_rows(k_rmsnorm<T, W, NV, kAny>, a, s, stream);
+  const size_t row = a.cols * sizeof(T) * (a.residual != nullptr ? 2 : 1);
+  if (a.rows <= s.grid * s.y || kStages * row * s.y > kRingMost)
+    return launch_rows(k_rmsnorm<T, W, NV, kFew>, a, s, stream);
+  s = shape_for(a.rows, a.cols, NV, row, false);
+  return launch_rows(k_rmsnorm<T, W, NV, kRing>, a, s, stream);
 }
 
 template <typename T, typename W>
-int launch_norm(const NormArgs &a, cudaStream_t stream) {
+int launch_norm(const NormArgs &a, bool plain, cudaStream_t stream) {
   switch (chunks_for(a.cols)) {
-    case 1: return launch_norm<T, W, 1>(a, stream);
-    case 2: return launch_norm<T, W, 2>(a, stream);
-    default: return launch_norm<T, W, 4>(a, stream);
+    case 1: return launch_norm<T, W, 1>(a, plain, stream);
+    case 2: return launch_norm<T, W, 2>(a, plain, stream);
+    default: return launch_norm<T, W, 4>(a, plain, stream);
   }
 }
 
 template <typename T, typename W, int NV>
-int launch_back(NormBackArgs a, int *grid, cudaStream_t stream) {
-  const int threads = threads_for(a.cols, NV), direct = ctas_for(a.rows, threads, 0);
-  const size_t ring = (size_t)kStages * a.cols * sizeof(T) * (a.dh != nullptr ? 3 : 2);
-  const bool use_ring = a.rows > direct && a.cols % 8 == 0 && a.dy_vec && a.h_vec &&
-                        (a.dh == nullptr || a.dh_vec) && ring <= kRingMost;
-  *grid = use_ring ? ctas_for(a.rows, threads, ring) : direct;
-  if (use_ring) return launch_rows(k_rmsnorm_back<T, W, NV, true>, a, *grid, threads, ring, stream);
-  return launch_rows(k_rmsnorm_back<T, W, NV, false>, a, *grid, threads, 0, stream);
+int launch_back(const NormBackArgs &a, bool plain, int *grid, cudaStream_t stream) {
+  const bool sums = a.parts != nullptr;
+  Shape s = shape_for(a.rows, a.cols, NV, 0, sums);
+  const size_t row = a.cols * sizeof(T) * (a.dh != nullptr ? 3 : 2);
+  const bool ring = plain && a.rows > s.grid * s.y && kStages * row * s.y <= kRingMost;
+  if (ring) s = shape_for(a.rows, a.cols, NV, row, sums);
+  *grid = s.grid;
+  if (ring) return launch_rows(k_rmsnorm_back<T, W, NV, kRing>, a, s, stream);
+  if (plain) return launch_rows(k_rmsnorm_back<T, W, NV, kFew>, a, s, stream);
+  return launch_rows(k_rmsnorm_back<T, W, NV, kAny>, a, s, stream);
 }
 
 template <typename T, typename W>
-int launch_back(const NormBackArgs &a, int *grid, cudaStream_t stream) {
+int launch_back(const NormBackArgs &a, bool plain, int *grid, cudaStream_t stream) {
   switch (chunks_for(a.cols)) {
-    case 1: return launch_back<T, W, 1>(a, grid, stream);
-    case 2: return launch_back<T, W, 2>(a, grid, stream);
-    default: return launch_back<T, W, 4>(a, grid, stream);
+    case 1: return launch_back<T, W, 1>(a, plain, grid, stream);
+    case 2: return launch_back<T, W, 2>(a, plain, grid, stream);
+    default: return launch_back<T, W, 4>(a, plain, grid, stream);
   }
 }
 
@@ -497,19 +572,18 @@ extern "C" int cmb_rmsnorm_e4m3_block128(const void *x, size_t ld_x, const void 
   if (current_cc() != 100)
     return fail(CMB_ERR_UNSUPPORTED, "%s: needs an sm_100 device (found cc %d)", fn, current_cc());
 
-  NormArgs a = {x, residual, weight, h, y, q, scale, rstd, ld_x, ld_residual, ld_h, ld_y, ld_q,
-                ld_scale, eps, rows, cols, false, false, false, false, false, false};
-  a.x_vec = b128::aligned_to(x, ld_x * elem, 16);
-  a.r_vec = b128::aligned_to(residual, ld_residual * elem, 16);
-  a.w_vec = b128::aligned_to(weight, 0, 16);
-  a.h_vec = b128::aligned_to(h, ld_h * elem, 16);
-  a.y_vec = b128::aligned_to(y, ld_y * elem, 16);
-  a.q_vec = b128::aligned_to(q, ld_q, 8);
+  const NormArgs a = {x, residual, weight, h, y, q, scale, rstd, ld_x, ld_residual, ld_h, ld_y,
+                      ld_q, ld_scale, eps, rows, cols, b128::aligned_to(q, ld_q, 8)};
+  const auto on16 = [&](const void *p, size_t ld) {
+    return p == nullptr || b128::aligned_to(p, ld * elem, 16);
+  };
+  const bool plain = cols % 8 == 0 && on16(x, ld_x) && on16(residual, ld_residual) &&
+                     on16(h, ld_h) && on16(y, ld_y);
   if (type == CMB_BF16)
-    return weight_type == CMB_BF16 ? launch_norm<__nv_bfloat16, __nv_bfloat16>(a, stream)
-                                   : launch_norm<__nv_bfloat16, float>(a, stream);
-  return weight_type == CMB_BF16 ? launch_norm<float, __nv_bfloat16>(a, stream)
-                                 : launch_norm<float, float>(a, stream);
+    return weight_type == CMB_BF16 ? launch_norm<__nv_bfloat16, __nv_bfloat16>(a, plain, stream)
+                                   : launch_norm<__nv_bfloat16, float>(a, plain, stream);
+  return weight_type == CMB_BF16 ? launch_norm<float, __nv_bfloat16>(a, plain, stream)
+                                 : launch_norm<float, float>(a, plain, stream);
 }
 
 extern "C" size_t cmb_rmsnorm_backward_workspace_bytes(int rows, int cols) {
@@ -553,22 +627,22 @@ extern "C" int cmb_rmsnorm_backward(const void *dy, size_t ld_dy, const void *h,
   if (current_cc() != 100)
     return fail(CMB_ERR_UNSUPPORTED, "%s: needs an sm_100 device (found cc %d)", fn, current_cc());
 
-  NormBackArgs a = {dy, h, dh, weight, rstd, dx,
-                    dweight != nullptr ? static_cast<float *>(workspace) : nullptr,
-                    ld_dy, ld_h, ld_dh, ld_dx, parts_pitch(cols), rows, cols,
-                    false, false, false, false, false};
-  a.dy_vec = b128::aligned_to(dy, ld_dy * elem, 16);
-  a.h_vec = b128::aligned_to(h, ld_h * elem, 16);
-  a.dh_vec = b128::aligned_to(dh, ld_dh * elem, 16);
-  a.w_vec = b128::aligned_to(weight, 0, 16);
-  a.dx_vec = b128::aligned_to(dx, ld_dx * elem, 16);
+  const NormBackArgs a = {dy, h, dh, weight, rstd, dx,
+                          dweight != nullptr ? static_cast<float *>(workspace) : nullptr,
+                          ld_dy, ld_h, ld_dh, ld_dx, parts_pitch(cols), rows, cols};
+  const auto on16 = [&](const void *p, size_t ld) {
+    return p == nullptr || b128::aligned_to(p, ld * elem, 16);
+  };
+  const bool plain = cols % 8 == 0 && on16(dy, ld_dy) && on16(h, ld_h) && on16(dh, ld_dh) &&
+                     on16(dx, ld_dx);
   int grid = 0;
   if (type == CMB_BF16)
-    rc = weight_type == CMB_BF16 ? launch_back<__nv_bfloat16, __nv_bfloat16>(a, &grid, stream)
-                                 : launch_back<__nv_bfloat16, float>(a, &grid, stream);
+    rc = weight_type == CMB_BF16
+             ? launch_back<__nv_bfloat16, __nv_bfloat16>(a, plain, &grid, stream)
+             : launch_back<__nv_bfloat16, float>(a, plain, &grid, stream);
   else
-    rc = weight_type == CMB_BF16 ? launch_back<float, __nv_bfloat16>(a, &grid, stream)
-                                 : launch_back<float, float>(a, &grid, stream);
+    rc = weight_type == CMB_BF16 ? launch_back<float, __nv_bfloat16>(a, plain, &grid, stream)
+                                 : launch_back<float, float>(a, plain, &grid, stream);
   if (rc || dweight == nullptr) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((cols + 31) / 32);

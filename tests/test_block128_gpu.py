@@ -107,7 +107,8 @@ def test_quantize(cuda, cmb, rows, cols, kind, block, which):
 
 @pytest.mark.parametrize("block", [1, 128])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("pitch,pad,offset", [(333, 3, 1), (336, 8, 0), (335, 0, 3), (344, 7, 8)])
+@pytest.mark.parametrize("pitch,pad,offset", [(333, 3, 1), (336, 8, 0), (335, 0, 3), (344, 7, 8),
+                                              (331, 6, 0)])
 def test_quantize_strides_and_alignment(cuda, cmb, kind, block, pitch, pad, offset):
     rng = np.random.default_rng(pitch)
     _, view = on_gpu(cuda, activations(rng, 131, 330), kind, pitch, offset)
@@ -387,9 +388,25 @@ def test_norm(cuda, cmb, rows, cols, kind, wkind, residual):
     assert np.array_equal(f64(x), keep[0])  # inputs stay
 
 
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(1200, 4096), (9000, 64), (5000, 1000), (5000, 1032),
+                                       (3000, 255), (2500, 2051), (1, 4601), (700, 8190),
+                                       (200, 30001)])
+def test_norm_more_rows_than_fit(cuda, cmb, rows, cols, kind, residual):
+    """Every width of CTA, several rows each, whole chunks and odd ones."""
+    rng = np.random.default_rng(rows + cols)
+    _, x = on_gpu(cuda, activations(rng, rows, cols), kind)
+    _, w = on_gpu(cuda, 1 + 0.1 * rng.normal(size=(1, cols)), "bf16")
+    r = on_gpu(cuda, 3 * rng.normal(size=(rows, cols)), kind)[1] if residual else None
+    keep = f64(x), f64(r) if residual else None
+    out = run_norm(cuda, cmb, x, r, w, kind, "bf16", 1e-5)
+    check_norm(out, *keep, f64(w)[0], kind, np.float32(1e-5))
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("cols,pitch,offset,pad", [(330, 333, 1, 3), (328, 336, 0, 8), (1000, 1001, 2, 1),
-                                                   (9000, 9003, 0, 5)])
+                                                   (9000, 9003, 0, 5), (513, 517, 3, 2), (7, 9, 1, 1)])
 def test_norm_strides_and_alignment(cuda, cmb, kind, cols, pitch, offset, pad):
     rng = np.random.default_rng(cols)
     _, x = on_gpu(cuda, activations(rng, 9, cols), kind, pitch, offset)
@@ -402,11 +419,12 @@ def test_norm_strides_and_alignment(cuda, cmb, kind, cols, pitch, offset, pad):
 
 @pytest.mark.parametrize("where", ["x", "r"])
 @pytest.mark.parametrize("rows", [3, 1000])
-def test_norm_residual_in_place(cuda, cmb, where, rows):
+@pytest.mark.parametrize("cols", [1544, 1547])
+def test_norm_residual_in_place(cuda, cmb, where, rows, cols):
     rng = np.random.default_rng(rows)
-    _, x = on_gpu(cuda, activations(rng, rows, 1544), "bf16")
-    _, r = on_gpu(cuda, rng.normal(size=(rows, 1544)), "bf16")
-    _, w = on_gpu(cuda, np.ones((1, 1544)), "bf16")
+    _, x = on_gpu(cuda, activations(rng, rows, cols), "bf16")
+    _, r = on_gpu(cuda, rng.normal(size=(rows, cols)), "bf16")
+    _, w = on_gpu(cuda, np.ones((1, cols)), "bf16")
     keep = f64(x), f64(r)
     out = run_norm(cuda, cmb, x, r, w, "bf16", "bf16", 1e-5, in_place=where)
     check_norm(out, *keep, f64(w)[0], "bf16", np.float32(1e-5))
@@ -505,8 +523,23 @@ def test_norm_backward(cuda, cmb, rows, cols, kind, wkind, residual):
                    kind)
 
 
+@pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("cols,pitch,offset,pad", [(330, 333, 1, 3), (328, 336, 0, 8), (1000, 1001, 2, 1)])
+@pytest.mark.parametrize("rows,cols", [(1200, 4096), (9000, 64), (5000, 1000), (5000, 1032),
+                                       (3000, 255), (2500, 2051), (1, 4601), (700, 8190),
+                                       (200, 30001)])
+def test_norm_backward_more_rows_than_fit(cuda, cmb, rows, cols, kind, residual):
+    rng = np.random.default_rng(rows + cols)
+    dy, h, dh, w, rstd = backward_inputs(cuda, rng, rows, cols, kind, "bf16")
+    dh = dh if residual else None
+    dx, grad = run_backward(cuda, cmb, dy, h, dh, w, rstd, kind, "bf16")
+    check_backward(dx, grad, f64(dy), f64(h), f64(dh) if residual else None, f64(w)[0], f64(rstd),
+                   kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("cols,pitch,offset,pad", [(330, 333, 1, 3), (328, 336, 0, 8), (1000, 1001, 2, 1),
+                                                   (513, 517, 3, 2), (7, 9, 1, 1)])
 def test_norm_backward_strides_and_alignment(cuda, cmb, kind, cols, pitch, offset, pad):
     rng = np.random.default_rng(cols)
     dy, h, dh, w, rstd = backward_inputs(cuda, rng, 40, cols, kind, "f32", pitch, offset)
@@ -515,9 +548,10 @@ def test_norm_backward_strides_and_alignment(cuda, cmb, kind, cols, pitch, offse
 
 
 @pytest.mark.parametrize("where", ["dy", "dh"])
-def test_norm_backward_in_place(cuda, cmb, where):
+@pytest.mark.parametrize("cols", [1544, 1547])
+def test_norm_backward_in_place(cuda, cmb, where, cols):
     rng = np.random.default_rng(2)
-    dy, h, dh, w, rstd = backward_inputs(cuda, rng, 900, 1544, "bf16", "bf16")
+    dy, h, dh, w, rstd = backward_inputs(cuda, rng, 900, cols, "bf16", "bf16")
     keep = [f64(t) for t in (dy, h, dh)]
     dx, grad = run_backward(cuda, cmb, dy, h, dh, w, rstd, "bf16", "bf16",
                             dx={"dy": dy, "dh": dh}[where])
