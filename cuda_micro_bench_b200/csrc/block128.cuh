@@ -75,54 +75,16 @@ __device__ __forceinline__ float max_magnitude(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z;\n\t"
-      "mov.b64 x, {%2, %3};\n\t"
-      "mov.b64 y, {%4, %5};\n\t"
-      "add.rn.f32x2 z, x, y;\n\t"
-      "mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
-// a * b + c, both halves at once.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z, w;\n\t"
-      "mov.b64 x, {%2, %3};\n\t"
-      "mov.b64 y, {%4, %5};\n\t"
-      "mov.b64 z, {%6, %7};\n\t"
-      "fma.rn.f32x2 w, x, y, z;\n\t"
-      "mov.b64 {%0, %1}, w; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-
-// a * s, both halves at once.
-__device__ __forceinline__ float2 mul2(float2 a, float2 s) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z;\n\t"
-      "mov.b64 x, {%2, %3};\n\t"
-      "mov.b64 y, {%4, %5};\n\t"
-      "mul.rn.f32x2 z, x, y;\n\t"
-      "mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(s.x), "f"(s.y));
-  return r;
-}
-
 // 8 values times `inv` as 8 e4m3 bytes.
 template <bool kAny>
-__device__ __forceinline__ uint2 e4m3x8(const float2 (&v)[4], float inv) {
-  const float2 s = make_float2(inv, inv);
-  float2 p[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = mul2(v[i], s);
-  return make_uint2(e4m3x4<kAny>(p[0].x, p[0].y, p[1].x, p[1].y),
-                    e4m3x4<kAny>(p[2].x, p[2].y, p[3].x, p[3].y));
+__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float inv) {
+  return make_uint2(e4m3x4<kAny>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                    e4m3x4<kAny>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+}
+// The rare form, out of the way of the other.
+static __device__ __noinline__ uint2 e4m3x8_any(float4 a, float4 b, float inv) {
+  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return e4m3x8<true>(v, inv);
 }
 
 // Both bf16 halves of a word times a bf16 each (given as fp32 bits' upper
@@ -252,12 +214,56 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack2(const Raw8<T> &r, float2 (&v)[4]) {
-  float u[8];
-  unpack(r, u);
+// a * b + c of both bf16 halves, in fp32: an instruction a value, with no
+// unpacking.
+__device__ __forceinline__ void fma_bf16x2(uint32_t a, uint32_t b, float &c0, float &c1) {
+  asm("{ .reg .b16 l, h, s, t;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "mov.b32 {s, t}, %3;\n\t"
+      "fma.rn.f32.bf16 %0, l, s, %0;\n\t"
+      "fma.rn.f32.bf16 %1, h, t, %1; }"
+      : "+f"(c0), "+f"(c1)
+      : "r"(a), "r"(b));
+}
+
+// c += a * b, element for element (exact products where both are bf16).
+__device__ __forceinline__ void fma8(const Raw8<__nv_bfloat16> &a, const Raw8<__nv_bfloat16> &b,
+                                     float (&c)[8]) {
+  fma_bf16x2(a.a.x, b.a.x, c[0], c[1]);
+  fma_bf16x2(a.a.y, b.a.y, c[2], c[3]);
+  fma_bf16x2(a.a.z, b.a.z, c[4], c[5]);
+  fma_bf16x2(a.a.w, b.a.w, c[6], c[7]);
+}
+template <typename A, typename B>
+__device__ __forceinline__ void fma8(const Raw8<A> &a, const Raw8<B> &b, float (&c)[8]) {
+  float u[8], v[8];
+  unpack(a, u);
+  unpack(b, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = make_float2(u[2 * i], u[2 * i + 1]);
+  for (int j = 0; j < 8; ++j) c[j] = fmaf(u[j], v[j], c[j]);
+}
+// The product alone; -0 leaves its sign.
+template <typename A, typename B>
+__device__ __forceinline__ void mul8(const Raw8<A> &a, const Raw8<B> &b, float (&c)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = -0.0f;
+  fma8(a, b, c);
+}
+
+// a + b.
+__device__ __forceinline__ void add8(const Raw8<__nv_bfloat16> &a, const Raw8<__nv_bfloat16> &b,
+                                     float (&c)[8]) {
+  const uint32_t one = 0x3F803F80u;
+  const Raw8<__nv_bfloat16> ones = {make_uint4(one, one, one, one)};
+  mul8(a, ones, c);
+  fma8(b, ones, c);
+}
+__device__ __forceinline__ void add8(const Raw8<float> &a, const Raw8<float> &b, float (&c)[8]) {
+  float u[8], v[8];
+  unpack(a, u);
+  unpack(b, v);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = u[j] + v[j];
 }
 
 // Rounded (nearest even) to the type of the row.
@@ -273,10 +279,9 @@ __device__ __forceinline__ void pack(const float (&v)[8], Raw8<float> &r) {
 }
 
 template <typename T>
-__device__ __forceinline__ Raw8<T> packed(const float2 (&v)[4]) {
-  const float u[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+__device__ __forceinline__ Raw8<T> packed(const float (&v)[8]) {
   Raw8<T> r;
-  pack(u, r);
+  pack(v, r);
   return r;
 }
 

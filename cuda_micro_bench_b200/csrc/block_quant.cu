@@ -37,8 +37,8 @@ __device__ __forceinline__ uint2 row_bytes(const Raw8<__nv_bfloat16> &r, float i
 }
 template <bool kAny>
 __device__ __forceinline__ uint2 row_bytes(const Raw8<float> &r, float inv) {
-  float2 v[4];
-  b128::unpack2(r, v);
+  float v[8];
+  b128::unpack(r, v);
   return b128::e4m3x8<kAny>(v, inv);
 }
 
@@ -135,8 +135,7 @@ __device__ __forceinline__ void column_bytes(const Raw8<float> (&raw)[8], int k,
       const int at = 2 * (k & 1) + d;
       v[i] = __uint_as_float(at == 0 ? r.x : at == 1 ? r.y : at == 2 ? r.z : r.w);
     }
-    const float2 u[4] = {{v[0], v[1]}, {v[2], v[3]}, {v[4], v[5]}, {v[6], v[7]}};
-    q[d] = b128::e4m3x8<kAny>(u, d == 0 ? inv0 : inv1);
+    q[d] = b128::e4m3x8<kAny>(v, d == 0 ? inv0 : inv1);
   }
 }
 

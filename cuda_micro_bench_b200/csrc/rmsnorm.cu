@@ -159,12 +159,12 @@ struct NormArgs {
 };
 
 // The e4m3 values and scales of 8 columns of a row; the whole warp.
+template <int kWay>
 __device__ __forceinline__ void store_quantized(const NormArgs &a, int row, int col, int n,
-                                                const float2 (&y)[4]) {
-  float top = b128::max_magnitude(y[0].x, y[0].y);
+                                                const float (&y)[8]) {
+  float top = b128::max_magnitude(y[0], y[1]);
 #pragma unroll
-  for (int j = 1; j < 4; ++j)
-    top = b128::max_magnitude(top, b128::max_magnitude(y[j].x, y[j].y));
+  for (int j = 2; j < 8; ++j) top = b128::max_magnitude(top, y[j]);
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1)
     top = b128::max_magnitude(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -172,16 +172,20 @@ __device__ __forceinline__ void store_quantized(const NormArgs &a, int row, int 
   if (any) {  // the scale is that of the finite values
     top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      top = fmaxf(top, fmaxf(b128::finite_magnitude(y[j].x), b128::finite_magnitude(y[j].y)));
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, b128::finite_magnitude(y[j]));
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
   const uint32_t byte = b128::scale_byte(top);
   const float inv = b128::scale_reciprocal(byte);
+  uint2 q = b128::e4m3x8<false>(y, inv);
+  if (any)
+    q = b128::e4m3x8_any(make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7]),
+                         inv);
   if (n > 0) {
-    b128::store_bytes(a.q + static_cast<size_t>(row) * a.ld_q + col,
-                      any ? b128::e4m3x8<true>(y, inv) : b128::e4m3x8<false>(y, inv), n, a.q_vec);
+    uint8_t *to = a.q + static_cast<size_t>(row) * a.ld_q + col;
+    if constexpr (kWay == kAny) b128::store_bytes(to, q, n, a.q_vec);
+    else *reinterpret_cast<uint2 *>(to) = q;
     if ((threadIdx.x & 15) == 0)
       a.scale[static_cast<size_t>(row) * a.ld_scale + col / b128::kBlock] =
           static_cast<uint8_t>(byte);
@@ -217,30 +221,28 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
     const int row = first + threadIdx.y;
     const bool here = row < a.rows;  // the same in a warp
     Raw8<T> h[NV];                   // as it is stored
-    float2 sq = make_float2(0.0f, 0.0f);
+    float sq[8] = {};
     if constexpr (kWay == kRing) ring.wait(turn);
     if (here) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
         h[i] = load_chunk<T, kWay>(ring, turn, 0, a.x, a.ld_x, row, col, n, in_x);
-        float2 v[4];
-        b128::unpack2(h[i], v);
         if (a.residual != nullptr) {
-          float2 u[4];
-          b128::unpack2(
-              load_chunk<T, kWay>(ring, turn, 1, a.residual, a.ld_r, row, col, n, in_r), u);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = b128::add2(v[j], u[j]);
+          float v[8];
+          b128::add8(h[i],
+                     load_chunk<T, kWay>(ring, turn, 1, a.residual, a.ld_r, row, col, n, in_r), v);
           h[i] = b128::packed<T>(v);
           store_chunk<T, kWay>(a.h, a.ld_h, row, col, n, h[i]);
-          b128::unpack2(h[i], v);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sq = b128::fma2(v[j], v[j], sq);
+        b128::fma8(h[i], h[i], sq);
       }
     }
-    const float sum = row_sum(sq.x + sq.y, part[turn & 1]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+      for (int j = 0; j < o; ++j) sq[j] += sq[j + o];
+    const float sum = row_sum(sq[0], part[turn & 1]);
     if constexpr (kWay == kRing)
       if (threadIdx.x == 0 && threadIdx.y == 0)
         ring.load(turn + kStages, a.rows);  // every thread has its chunks
@@ -250,16 +252,14 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      float2 y[4], w[4];
-      b128::unpack2(h[i], y);
-      b128::unpack2(weight.chunk(i), w);
+      float y[8];
+      b128::mul8(h[i], weight.chunk(i), y);
       // behind the row's end h is 0 and y too, or NaN where rstd is not finite,
       // which a block's scale passes over
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        y[j] = b128::mul2(b128::mul2(y[j], make_float2(rstd, rstd)), w[j]);
+      for (int j = 0; j < 8; ++j) y[j] *= rstd;
       if (a.y != nullptr) store_chunk<T, kWay>(a.y, a.ld_y, row, col, n, b128::packed<T>(y));
-      if (a.q != nullptr) store_quantized(a, row, col, n, y);
+      if (a.q != nullptr) store_quantized<kWay>(a, row, col, n, y);
     }
   }
 }
@@ -301,56 +301,49 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
     in_dh = Bounds::of(static_cast<const T *>(a.dh), a.ld_dh, a.rows, a.cols);
   }
   const Weight<W, NV> weight(a.weight, a.cols);
-  float2 dw[NV][4] = {};
+  float dw[NV][8] = {};
   int turn = 0;
   for (int first = blockIdx.x * blockDim.y; first < a.rows;
        first += gridDim.x * blockDim.y, ++turn) {
     const int row = first + threadIdx.y;
     const bool here = row < a.rows;  // the same in a warp
     const float rstd = here ? a.rstd[row] : 0.0f;
-    const float2 rstd2 = make_float2(rstd, rstd);
-    float2 along = make_float2(0.0f, 0.0f);
+    float along = 0.0f;  // sum of g h
     if constexpr (kWay == kRing) ring.wait(turn);
     if (here) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-        float2 g[4], u[4], w[4];
-        b128::unpack2(load_chunk<T, kWay>(ring, turn, 0, a.dy, a.ld_dy, row, col, n, in_dy), g);
-        b128::unpack2(load_chunk<T, kWay>(ring, turn, 1, a.h, a.ld_h, row, col, n, in_h), u);
-        b128::unpack2(weight.chunk(i), w);
-        if (n > 0) {  // behind the row's end 0 * rstd may be NaN
+        if (n <= 0) continue;
+        float p[8], w[8];  // dy h
+        b128::mul8(load_chunk<T, kWay>(ring, turn, 0, a.dy, a.ld_dy, row, col, n, in_dy),
+                   load_chunk<T, kWay>(ring, turn, 1, a.h, a.ld_h, row, col, n, in_h), p);
+        b128::unpack(weight.chunk(i), w);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            u[j] = b128::mul2(u[j], rstd2);
-            if (kWay == kAny && n < 8) {
-              if (2 * j >= n) u[j].x = 0.0f;
-              if (2 * j + 1 >= n) u[j].y = 0.0f;
-            }
-            dw[i][j] = b128::fma2(g[j], u[j], dw[i][j]);
-            along = b128::fma2(b128::mul2(g[j], w[j]), u[j], along);
-          }
+        for (int j = 0; j < 8; ++j) {
+          dw[i][j] = fmaf(p[j], rstd, dw[i][j]);
+          along = fmaf(p[j], w[j], along);
         }
       }
     }
-    const float mean = row_sum(along.x + along.y, part[turn & 1]) / static_cast<float>(a.cols);
+    const float sum = row_sum(along, part[turn & 1]);
     // every thread is past the last turn: its place takes another
     if constexpr (kWay == kRing)
       if (threadIdx.x == 0 && threadIdx.y == 0 && turn > 0) ring.load(turn - 1 + kStages, a.rows);
     if (!here) continue;
-    const float2 minus = make_float2(-rstd * mean, -rstd * mean);
+    // dx = rstd g - h rstd^3 mean(g h) + dh
+    const float minus = -rstd * rstd * (rstd * (sum / static_cast<float>(a.cols)));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
-      float2 g[4], u[4], w[4], past[4] = {};
-      b128::unpack2(load_chunk<T, kWay>(ring, turn, 0, a.dy, a.ld_dy, row, col, n, in_dy), g);
-      b128::unpack2(load_chunk<T, kWay>(ring, turn, 1, a.h, a.ld_h, row, col, n, in_h), u);
+      float g[8], u[8], past[8] = {};
+      b128::mul8(load_chunk<T, kWay>(ring, turn, 0, a.dy, a.ld_dy, row, col, n, in_dy),
+                 weight.chunk(i), g);
+      b128::unpack(load_chunk<T, kWay>(ring, turn, 1, a.h, a.ld_h, row, col, n, in_h), u);
       if (a.dh != nullptr)
-        b128::unpack2(load_chunk<T, kWay>(ring, turn, 2, a.dh, a.ld_dh, row, col, n, in_dh), past);
-      b128::unpack2(weight.chunk(i), w);
+        b128::unpack(load_chunk<T, kWay>(ring, turn, 2, a.dh, a.ld_dh, row, col, n, in_dh), past);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        g[j] = b128::fma2(rstd2, b128::fma2(u[j], minus, b128::mul2(g[j], w[j])), past[j]);
+      for (int j = 0; j < 8; ++j) g[j] = fmaf(rstd, g[j], fmaf(u[j], minus, past[j]));
       store_chunk<T, kWay>(a.dx, a.ld_dx, row, col, n, b128::packed<T>(g));
     }
   }
@@ -364,8 +357,8 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int chunk = i * blockDim.x + threadIdx.x;
-      float4 v[2] = {{dw[i][0].x, dw[i][0].y, dw[i][1].x, dw[i][1].y},
-                     {dw[i][2].x, dw[i][2].y, dw[i][3].x, dw[i][3].y}};
+      float4 v[2] = {{dw[i][0], dw[i][1], dw[i][2], dw[i][3]},
+                     {dw[i][4], dw[i][5], dw[i][6], dw[i][7]}};
       if (chunk * 8 >= a.cols) continue;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -463,7 +456,8 @@ int launch_rows(void (*kernel)(A), const A &a, const Shape &s, cudaStream_t stre
   return CMB_OK;
 }
 
-// `plain`: every row of every matrix starts on 16 bytes, and cols % 8 == 0.
+// `plain`: every row of every matrix starts on 16 bytes (of q on 8), and cols
+// % 8 == 0.
 template <typename T, typename W, int NV>
 int launch_norm(const NormArgs &a, bool plain, cudaStream_t stream) {
   Shape s = shape_for(a.rows, a.cols, NV, 0, false);
@@ -578,7 +572,7 @@ extern "C" int cmb_rmsnorm_e4m3_block128(const void *x, size_t ld_x, const void 
     return p == nullptr || b128::aligned_to(p, ld * elem, 16);
   };
   const bool plain = cols % 8 == 0 && on16(x, ld_x) && on16(residual, ld_residual) &&
-                     on16(h, ld_h) && on16(y, ld_y);
+                     on16(h, ld_h) && on16(y, ld_y) && a.q_vec;
   if (type == CMB_BF16)
     return weight_type == CMB_BF16 ? launch_norm<__nv_bfloat16, __nv_bfloat16>(a, plain, stream)
                                    : launch_norm<__nv_bfloat16, float>(a, plain, stream);
