@@ -416,6 +416,10 @@ __device__ __forceinline__ void store_bytes(uint8_t *p, uint2 q, int n, bool ali
 
 // ------------------------------------------------------------ host checks
 
+// Rows and columns stay far enough under 2^31 that an index one tile or one
+// round of CTAs past the end is still an int.
+constexpr int kMostExtent = 0x7FFF0000;
+
 inline bool aligned_to(const void *p, size_t pitch_bytes, size_t to) {
   return (reinterpret_cast<uintptr_t>(p) % to) == 0 && pitch_bytes % to == 0;
 }

@@ -340,7 +340,7 @@ extern "C" int cmb_quantize_e4m3_block128(const void *src, int src_type, int row
     return fail(CMB_ERR_INVALID_ARG, "%s: src_type %d is not CMB_BF16 or CMB_F32", fn, src_type);
   if (block_rows != 1 && block_rows != kBlock)
     return fail(CMB_ERR_INVALID_ARG, "%s: block_rows %d not 1 or 128", fn, block_rows);
-  if (rows < 0 || cols < 0)
+  if (rows < 0 || cols < 0 || rows > b128::kMostExtent || cols > b128::kMostExtent)
     return fail(CMB_ERR_INVALID_ARG, "%s: %d x %d values", fn, rows, cols);
   if ((dst == nullptr) != (scale == nullptr) || (dst_t == nullptr) != (scale_t == nullptr))
     return fail(CMB_ERR_INVALID_ARG, "%s: values and scales go together", fn);

@@ -524,7 +524,7 @@ int check_types(const char *fn, int type, int weight_type, int rows, int cols) {
   if ((type != CMB_BF16 && type != CMB_F32) || (weight_type != CMB_BF16 && weight_type != CMB_F32))
     return fail(CMB_ERR_INVALID_ARG, "%s: types %d, %d are not CMB_BF16 or CMB_F32", fn, type,
                 weight_type);
-  if (rows < 0 || cols <= 0 || cols > CMB_RMSNORM_MAX_COLS)
+  if (rows < 0 || rows > b128::kMostExtent || cols <= 0 || cols > CMB_RMSNORM_MAX_COLS)
     return fail(CMB_ERR_INVALID_ARG, "%s: %d rows of %d columns (1-%d)", fn, rows, cols,
                 CMB_RMSNORM_MAX_COLS);
   return CMB_OK;

@@ -35,6 +35,7 @@ QUANT = dict(src=P, src_type=BF16, rows=4, cols=300, ld_src=300, block_rows=1, d
     (dict(src_type=2), "src_type"), (dict(src_type=-1), "src_type"),
     (dict(block_rows=0), "block_rows"), (dict(block_rows=64), "block_rows"),
     (dict(rows=-1), "values"), (dict(cols=-4), "values"),
+    (dict(rows=2**31 - 1), "values"), (dict(cols=2**31 - 1), "values"),
     (dict(scale=None), "together"), (dict(dst=None), "together"), (dict(dst_t=None), "together"),
     (dict(scale_t=None), "together"),
     (dict(dst=None, scale=None, dst_t=None, scale_t=None), "nothing"),
@@ -51,7 +52,8 @@ GEMM = dict(A=P, lda=304, sa=P, ld_sa=3, B=P, ldb=304, sb=P, ld_sb=3, block_rows
 
 @pytest.mark.parametrize("change,word", [
     (dict(c_type=3), "c_type"), (dict(block_rows_b=2), "block_rows_b"), (dict(M=-1), "M -1"),
-    (dict(N=-1), "N -1"), (dict(K=-1), "K -1"), (dict(status=Q), "status"), (dict(C=None), "C is"),
+    (dict(N=-1), "N -1"), (dict(K=-1), "K -1"), (dict(M=2**31 - 1), "M 2147483647"),
+    (dict(N=2**31 - 1), "N 2147483647"), (dict(K=2**31 - 1), "K 2147483647"), (dict(status=Q), "status"), (dict(C=None), "C is"),
     (dict(C=Q), "C is"), (dict(C=ctypes.c_void_p(4098), c_type=F32), "C is"),
     (dict(ldc=199), "ldc"), (dict(A=None), "null"), (dict(B=None), "null"), (dict(sa=None), "null"),
     (dict(sb=None), "null"), (dict(A=ctypes.c_void_p(4104)), "16-byte"), (dict(lda=312), "16"),
@@ -68,6 +70,7 @@ NORM = dict(x=P, ld_x=300, residual=P, ld_residual=300, type=BF16, weight=P, wei
 
 @pytest.mark.parametrize("change,word", [
     (dict(type=2), "types"), (dict(weight_type=7), "types"), (dict(rows=-1), "rows"),
+    (dict(rows=2**31 - 1), "rows"),
     (dict(cols=0), "columns"), (dict(cols=32769), "columns"), (dict(eps=ctypes.c_float(-1)), "eps"),
     (dict(eps=ctypes.c_float(float("nan"))), "eps"), (dict(q=None), "together"),
     (dict(scale=None), "together"), (dict(residual=None), "together"), (dict(h=None), "together"),
