@@ -261,17 +261,11 @@ void parallel_for(int n, F fn) {
 // the stated "rel tol 1e-2".  Each fp64 product is summed in k order; the
 // tile's B columns are decoded once (k-major) and the row blocks are spread
 // over the host's threads.
-template <bool kFp8>
-double sampled_gemm_error(const std::vector<uint8_t> &A, const std::vector<uint8_t> &B,
-                          const std::vector<float> &C, int M, int N, int K, double sa, double sb,
+// a(row, k) and b(row, k) give the operands' values.
+template <class FA, class FB>
+double sampled_tile_error(FA a_at, FB b_at, const std::vector<float> &C, int M, int N, int K,
                           int tiles) {
   constexpr int T = 256, RB = 4, CB = 16;
-  auto elem = [&](const std::vector<uint8_t> &X, size_t i, double s) -> double {
-    if (kFp8) return e4m3_to_float(X[i]) * s;
-    uint16_t v;
-    std::memcpy(&v, &X[2 * i], 2);
-    return bf16_bits_to_float(v);
-  };
   double worst = 0.0;
   uint64_t r = 12345;
   std::vector<double> bt((size_t)K * T), ref((size_t)T * T);
@@ -282,12 +276,12 @@ double sampled_gemm_error(const std::vector<uint8_t> &A, const std::vector<uint8
     if (t == 0) r0 = c0 = 0;
     if (t == 1) r0 = M - T, c0 = N - T;
     parallel_for(K, [&](int k) {
-      for (int j = 0; j < T; ++j) bt[(size_t)k * T + j] = elem(B, (size_t)(c0 + j) * K + k, sb);
+      for (int j = 0; j < T; ++j) bt[(size_t)k * T + j] = b_at(c0 + j, k);
     });
     parallel_for(T / RB, [&](int blk) {
       std::vector<double> a((size_t)RB * K);
       for (int q = 0; q < RB; ++q)
-        for (int k = 0; k < K; ++k) a[(size_t)q * K + k] = elem(A, (size_t)(r0 + blk * RB + q) * K + k, sa);
+        for (int k = 0; k < K; ++k) a[(size_t)q * K + k] = a_at(r0 + blk * RB + q, k);
       for (int j0 = 0; j0 < T; j0 += CB) {
         double acc[RB][CB] = {};
         for (int k = 0; k < K; ++k) {
@@ -312,6 +306,22 @@ double sampled_gemm_error(const std::vector<uint8_t> &A, const std::vector<uint8
     worst = std::max(worst, err_max / std::max(ref_max, 1e-300));
   }
   return worst;
+}
+
+// The same for one scale per operand.
+template <bool kFp8>
+double sampled_gemm_error(const std::vector<uint8_t> &A, const std::vector<uint8_t> &B,
+                          const std::vector<float> &C, int M, int N, int K, double sa, double sb,
+                          int tiles) {
+  auto elem = [K](const std::vector<uint8_t> &X, int row, int k, double s) -> double {
+    const size_t i = (size_t)row * K + k;
+    if (kFp8) return e4m3_to_float(X[i]) * s;
+    uint16_t v;
+    std::memcpy(&v, &X[2 * i], 2);
+    return bf16_bits_to_float(v);
+  };
+  return sampled_tile_error([&](int r, int k) { return elem(A, r, k, sa); },
+                            [&](int r, int k) { return elem(B, r, k, sb); }, C, M, N, K, tiles);
 }
 
 }  // namespace
@@ -760,6 +770,147 @@ int section_tensor_core() {
   return CMB_OK;
 }
 
+namespace {
+
+// The calls of one e4m3 linear layer of 8192 tokens x 8192 x 8192 with a scale
+// for each block of 128 values: norm with residual, product, the norm's
+// gradient; each timed and checked on samples against fp64.
+int fp8_linear_layer() {
+  const int n = 8192, groups = n / 128;
+  const size_t nn = (size_t)n * n;
+  const float eps = 1e-5f;
+  DevBuf x, r, h, w, gain, xq, xs, wq, ws, c, rstd, dx, dgain, room, st;
+  TRY(x.alloc(nn * 2));
+  TRY(r.alloc(nn * 2));
+  TRY(h.alloc(nn * 2));
+  TRY(w.alloc(nn * 2));
+  TRY(dx.alloc(nn * 2));
+  TRY(gain.alloc(n * 2));
+  TRY(xq.alloc(nn));
+  TRY(xs.alloc((size_t)n * groups));
+  TRY(wq.alloc(nn));
+  TRY(ws.alloc((size_t)groups * groups));
+  TRY(c.alloc(nn * 4));
+  TRY(rstd.alloc(n * sizeof(float)));
+  TRY(dgain.alloc(n * sizeof(float)));
+  const size_t room_bytes = cmb_rmsnorm_backward_workspace_bytes(n, n);
+  TRY(room.alloc(room_bytes));
+  TRY(st.alloc(sizeof(int)));
+  CMB_CUDA_TRY(cudaMemset(st.p, 0, sizeof(int)));
+  TRY(cmb_fill_normal_bf16(x.as<uint16_t>(), nn, kGemmSeed + 2, 1.0f, nullptr));
+  TRY(cmb_fill_normal_bf16(r.as<uint16_t>(), nn, kGemmSeed + 3, 3.0f, nullptr));
+  TRY(cmb_fill_normal_bf16(w.as<uint16_t>(), nn, kGemmSeed + 4, 1.0f / std::sqrt((float)n), nullptr));
+  TRY(cmb_fill_normal_bf16(gain.as<uint16_t>(), n, kGemmSeed + 5, 1.0f, nullptr));
+
+  double ms_q = 0, ms_n = 0, ms_g = 0, ms_b = 0;
+  TRY(time_median(
+      [&] {
+        return cmb_quantize_e4m3_block128(w.p, CMB_BF16, n, n, n, 128, wq.as<uint8_t>(), n,
+                                          ws.as<uint8_t>(), groups, nullptr, 0, nullptr, 0, nullptr);
+      },
+      6, 1, &ms_q));
+  TRY(time_median(
+      [&] {
+        return cmb_rmsnorm_e4m3_block128(x.p, n, r.p, n, CMB_BF16, gain.p, CMB_BF16, eps, n, n, h.p,
+                                         n, nullptr, 0, xq.as<uint8_t>(), n, xs.as<uint8_t>(),
+                                         groups, rstd.as<float>(), nullptr);
+      },
+      6, 1, &ms_n));
+  TRY(time_median(
+      [&] {
+        return cmb_gemm_e4m3_block128(xq.as<uint8_t>(), n, xs.as<uint8_t>(), groups,
+                                      wq.as<uint8_t>(), n, ws.as<uint8_t>(), groups, 128, c.p, n,
+                                      CMB_F32, n, n, n, st.as<int>(), nullptr);
+      },
+      6, 1, &ms_g));
+  TRY(time_median(
+      [&] {
+        return cmb_rmsnorm_backward(r.p, n, h.p, n, x.p, n, CMB_BF16, gain.p, CMB_BF16,
+                                    rstd.as<float>(), n, n, dx.p, n, dgain.as<float>(), room.p,
+                                    room_bytes, nullptr);
+      },
+      6, 1, &ms_b));
+  int status = 0;
+  CMB_CUDA_TRY(cudaMemcpy(&status, st.p, sizeof(status), cudaMemcpyDeviceToHost));
+  if (status != 0) return fail(status, "block-scaled GEMM: a bounded wait expired");
+
+  std::vector<uint8_t> hxq(nn), hxs((size_t)n * groups), hwq(nn), hws((size_t)groups * groups);
+  std::vector<float> hc(nn);
+  CMB_CUDA_TRY(cudaMemcpy(hxq.data(), xq.p, hxq.size(), cudaMemcpyDeviceToHost));
+  CMB_CUDA_TRY(cudaMemcpy(hxs.data(), xs.p, hxs.size(), cudaMemcpyDeviceToHost));
+  CMB_CUDA_TRY(cudaMemcpy(hwq.data(), wq.p, hwq.size(), cudaMemcpyDeviceToHost));
+  CMB_CUDA_TRY(cudaMemcpy(hws.data(), ws.p, hws.size(), cudaMemcpyDeviceToHost));
+  CMB_CUDA_TRY(cudaMemcpy(hc.data(), c.p, nn * 4, cudaMemcpyDeviceToHost));
+  const double err = sampled_tile_error(
+      [&](int row, int k) {
+        return e4m3_to_float(hxq[(size_t)row * n + k]) *
+               std::ldexp(1.0, hxs[(size_t)row * groups + k / 128] - 127);
+      },
+      [&](int row, int k) {
+        return e4m3_to_float(hwq[(size_t)row * n + k]) *
+               std::ldexp(1.0, hws[(size_t)(row / 128) * groups + k / 128] - 127);
+      },
+      hc, n, n, n, 8);
+  if (err > 1e-2)
+    return fail(CMB_ERR_MISMATCH, "block-scaled GEMM: sampled rel err %.3g > 1e-2", err);
+
+  // Four rows of the norm and of its gradient against fp64: e4m3 is off by at
+  // most 2^-4 of a value or half a subnormal step, bf16 by 2^-8, and the fp32
+  // statistics by far less.
+  std::vector<uint16_t> row_x(n), row_r(n), row_h(n), row_d(n), g(n);
+  CMB_CUDA_TRY(cudaMemcpy(g.data(), gain.p, n * 2, cudaMemcpyDeviceToHost));
+  for (int i = 0; i < 4; ++i) {
+    const size_t at = (size_t)(i * 2730) * n;
+    auto fetch = [&](std::vector<uint16_t> &to, const DevBuf &from) {
+      return cudaMemcpy(to.data(), static_cast<const uint16_t *>(from.p) + at, n * 2,
+                        cudaMemcpyDeviceToHost);
+    };
+    CMB_CUDA_TRY(fetch(row_x, x));
+    CMB_CUDA_TRY(fetch(row_r, r));
+    CMB_CUDA_TRY(fetch(row_h, h));
+    CMB_CUDA_TRY(fetch(row_d, dx));
+    double sq = 0, along = 0;
+    for (int k = 0; k < n; ++k) {
+      const double v = bf16_bits_to_float(row_h[k]);
+      const double sum = (double)bf16_bits_to_float(row_x[k]) + bf16_bits_to_float(row_r[k]);
+      if (std::fabs(v - sum) > std::ldexp(std::fabs(sum), -8) * 1.001)
+        return fail(CMB_ERR_MISMATCH, "rmsnorm: h = %g for a sum of %g", v, sum);
+      sq += v * v;
+      along += (double)bf16_bits_to_float(row_r[k]) * bf16_bits_to_float(g[k]) * v;
+    }
+    const double rs = 1.0 / std::sqrt(sq / n + eps);
+    for (int k = 0; k < n; ++k) {
+      const double v = bf16_bits_to_float(row_h[k]), gk = bf16_bits_to_float(g[k]);
+      const double y = v * rs * gk;
+      const double s = std::ldexp(1.0, hxs[at / n * groups + k / 128] - 127);
+      const double got = e4m3_to_float(hxq[at + k]) * s;
+      if (std::fabs(got - y) > std::max(std::fabs(y) / 16, s / 1024) * 1.001)
+        return fail(CMB_ERR_MISMATCH, "rmsnorm: %g for y = %g", got, y);
+      const double dy = bf16_bits_to_float(row_r[k]), past = bf16_bits_to_float(row_x[k]);
+      const double d = rs * (dy * gk - v * rs * rs * along / n) + past;
+      const double room_d = std::ldexp(std::fabs(d), -8) +
+                            1e-5 * (std::fabs(rs * dy * gk) + std::fabs(past) + std::fabs(v));
+      if (std::fabs(bf16_bits_to_float(row_d[k]) - d) > room_d * 1.001)
+        return fail(CMB_ERR_MISMATCH, "rmsnorm backward: %g for dx = %g",
+                    (double)bf16_bits_to_float(row_d[k]), d);
+    }
+  }
+  const double tf = 2.0 * n * nn / (ms_g * 1e-3) / 1e12;
+  const double gq = 3.0 * nn / (ms_q * 1e-3) / 1e9, gn = 7.0 * nn / (ms_n * 1e-3) / 1e9,
+               gb = 8.0 * nn / (ms_b * 1e-3) / 1e9;
+  printf("  e4m3 with a scale per block of 128, 8192^3: GEMM %.1f TFLOP/s (sampled rel err %.1e), "
+         "quantise %.0f GB/s, RMS norm %.0f GB/s, its gradient %.0f GB/s\n", tf, err, gq, gn, gb);
+  g_results.log("fp8_block128", "gemm_8192_tflops", tf, "TFLOP/s");
+  g_results.log("fp8_block128", "gemm_8192_max_rel_err", err, "");
+  g_results.log("fp8_block128", "quantize_8192_gbps", gq, "GB/s");
+  g_results.log("fp8_block128", "rmsnorm_8192_gbps", gn, "GB/s");
+  g_results.log("fp8_block128", "rmsnorm_backward_8192_gbps", gb, "GB/s");
+  g_results.log("fp8_block128", "verified", 1.0, "bool");
+  return CMB_OK;
+}
+
+}  // namespace
+
 int section_tensor_core_extended() {
   DeviceInfo info;
   TRY(query_device(0, &info));
@@ -903,7 +1054,7 @@ int section_tensor_core_extended() {
     g_results.log("tensor_core_tcgen05", p + "_bf16out_tflops", tfb, "TFLOP/s");
     g_results.log("tensor_core_tcgen05", p + "_bf16out_verified", 1.0, "bool");
   }
-  return CMB_OK;
+  return fp8_linear_layer();
 }
 
 namespace {

@@ -163,6 +163,14 @@ def check(doc, full=True, keys=None):
     for k in ("sum_gbps", "memcpy_gbps", "chase_ns_per_hop", "gemm_fp64_tiles_tflops"):
         bound("host_ref", k, 0, 1e6, "a positive host timing")
     # the die map: every SM on one of two dies, far loads slower than near
+    # the block-scaled e4m3 layer: products under the peak, streams under HBM's
+    bound("fp8_block128", "gemm_8192_tflops", 0, B200["fp8_tflops"] * 1.05, "dense tensor peak")
+    for key in ("quantize_8192_gbps", "rmsnorm_8192_gbps", "rmsnorm_backward_8192_gbps"):
+        bound("fp8_block128", key, 0, hbm, "HBM3e bandwidth")
+    flag("fp8_block128", "verified")
+    err = val("fp8_block128", "gemm_8192_max_rel_err")
+    if err is not None and err > 1e-2:
+        fail(f"fp8_block128.gemm_8192_max_rel_err = {err} above 1e-2")
     dies = [val("tensor_core_tcgen05", f"sms_on_die{d}") for d in (0, 1)]
     if all(x is not None for x in dies) and (min(dies) <= 0 or sum(dies) != B200["sm_count"]):
         fail(f"tensor_core_tcgen05.sms_on_die0/1 = {dies[0]} / {dies[1]}: not a split of "

@@ -161,3 +161,20 @@ def test_reference_gradient_matches_differences():
         e = np.zeros_like(w)
         e[j] = d
         assert abs((loss(h, w + e) - loss(h, w - e)) / (2 * d) - dw[j]) < 1e-7
+
+
+def test_validator_knows_the_layer():
+    from cuda_micro_bench_b200 import validate_results
+
+    def problems(**change):
+        v = dict(gemm_8192_tflops=2700.0, gemm_8192_max_rel_err=1e-6, quantize_8192_gbps=5000.0,
+                 rmsnorm_8192_gbps=5900.0, rmsnorm_backward_8192_gbps=5900.0, verified=1.0)
+        v.update(change)
+        doc = {"device": "NVIDIA B200", "architecture": "10.0", "sm_count": 148,
+               "results": {"fp8_block128": {k: {"value": x, "unit": ""} for k, x in v.items()}}}
+        return validate_results.check(doc, full=False)
+
+    assert problems() == []
+    for change in (dict(gemm_8192_tflops=5000.0), dict(rmsnorm_8192_gbps=9000.0),
+                   dict(verified=0.0), dict(gemm_8192_max_rel_err=0.5)):
+        assert len(problems(**change)) == 1, change

@@ -737,3 +737,25 @@ def test_layer_in_a_graph_and_on_a_stream(cuda, cmb, tokens):
         for name, t in L.outputs().items():
             assert cuda.equal(t, E.outputs()[name]), name
     assert int(L.status.item()) == 0
+
+
+def test_command_line_runs_and_checks_the_layer(cuda, tmp_path):
+    """`--tensor-ext` times the operators at 8192^3, checks samples of each
+    against fp64 and logs what the validator accepts."""
+    import json
+    import os
+    import subprocess
+
+    from cuda_micro_bench_b200 import validate_results
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = tmp_path / "results.json"
+    p = subprocess.run([os.path.join(root, "cuda_micro_bench_b200", "bin", "cmb_b200"),
+                        "--tensor-ext", f"--out={out}"], capture_output=True, text=True, timeout=600)
+    assert p.returncode == 0, p.stdout[-2000:] + p.stderr[-2000:]
+    doc = json.loads(out.read_text())
+    got = doc["results"]["fp8_block128"]
+    assert set(got) == {"gemm_8192_tflops", "gemm_8192_max_rel_err", "quantize_8192_gbps",
+                        "rmsnorm_8192_gbps", "rmsnorm_backward_8192_gbps", "verified"}
+    assert got["verified"]["value"] == 1.0
+    assert [m for m in validate_results.check(doc, full=False) if "fp8_block128" in m] == []
