@@ -22,6 +22,12 @@
 // each MMA names the byte of the word its K block is.  Both places have two
 // buffers.
 //
+// The tensor core adds to its fp32 accumulator by truncation, so a sum's error
+// grows with K: 5.5e-7 of C (2-norm) at K = 2048, 2.7e-6 at 8192, against 3.6e-7
+// for the same sums rounded to nearest.  A bf16 C does not show it; for an fp32 C
+// an accumulator takes at most 16 K blocks (kSumBlocks) and the parts are added
+// in registers, rounded to nearest.
+//
 // Two kernels: k_gemm_pair for many tokens (tensor core and L2 delivery
 // bound), k_gemm_split for few (bound by reading the weights once).
 #include <cuda.h>
@@ -56,6 +62,7 @@ struct Args {
   int stages;
   int split;                 // CTAs that share a tile's K (k_gemm_split)
   int tmem_cols;             // TMEM columns to allocate (k_gemm_split)
+  int sums;                  // accumulators that share a CTA's K (k_gemm_split)
   int *status;
 };
 
@@ -67,6 +74,7 @@ constexpr int kScaleCol = 480;          // TMEM columns of the scales: 2 x 4 and
 constexpr size_t kSmemMost = 227 * 1024 - 1024;  // less what is static
 constexpr size_t kSmemHalf = 112 * 1024;         // two CTAs a SM
 constexpr int kSplitThreads = 256;
+constexpr int kSumBlocks = 16;  // K blocks of an accumulator where C is fp32
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d) {
@@ -262,6 +270,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = uniform(tmem_holder);
+  const int each = (kb1 - kb0 + g.sums - 1) / g.sums;  // K blocks of an accumulator
   const Waiter wait{&abort_flag, g.status};
   dev::grid_dep_wait();
   dev::grid_dep_launch();
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                                100000000ull);
       }
   } else if (warp == 1) {
-    int s = 0, i = 0;
+    int s = 0, i = 0, sum = 0, left = each;
     uint32_t ph = 0;
     bool ok = true;
     for (int b = kb0 >> 2; b <= (kb1 - 1) >> 2 && ok; ++b, ++i) {
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       if (!wait(&bdone[slot], ((i >> 1) & 1) ^ 1)) break;
       tc::fence_after_sync();
       const uint32_t words = dev::smem_addr(scales + (4 * buf + (b & 3)) * kSplitSlot);
-      const uint32_t sf_w = tmem + g.n + 4 * slot, sf_t = tmem + g.n + 8 + 4 * slot;
+      const uint32_t sf_w = tmem + g.sums * g.n + 4 * slot, sf_t = sf_w + 8;
       if (dev::elect_one()) {
         tc::cp_scales<1>(sf_w, tc::rows16_desc(words));
         tc::cp_scales<1>(sf_t, tc::rows16_desc(words + 512));
@@ -317,15 +326,18 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         const uint32_t w = dev::smem_addr(ring + (size_t)s * stage_bytes);
         const uint64_t dw = tc::sw128_kmajor_desc(w), dt = tc::sw128_kmajor_desc(w + kWBytes);
         const uint32_t idesc = tc::instr_desc_block_scaled(128, g.n, kb & 3);
+        const uint32_t d = tmem + sum * g.n;
+        const bool first = left == each;  // of its accumulator
         if (dev::elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc::mma_block_scaled<1>(tmem, dw + 2 * k, dt + 2 * k, idesc, sf_w, sf_t,
-                                    (kb != kb0 || k != 0) ? 1u : 0u);
+            tc::mma_block_scaled<1>(d, dw + 2 * k, dt + 2 * k, idesc, sf_w, sf_t,
+                                    (!first || k != 0) ? 1u : 0u);
           tc::commit<1>(dev::smem_addr(&empty[s]));
         }
         __syncwarp();
         if (++s == g.stages) s = 0, ph ^= 1;
+        if (--left == 0) left = each, ++sum;
       }
       if (dev::elect_one()) {
         tc::commit<1>(dev::smem_addr(&bdone[slot]));
@@ -361,8 +373,18 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     float *mine = reinterpret_cast<float *>(ring) + row;
     for (int c0 = 0; c0 < g.n && ok; c0 += 16) {
       uint32_t r[16];
-      tc::ld_32x32b_x16(tmem + (static_cast<uint32_t>(row & 96) << 16) + c0, r);
+      const uint32_t at = tmem + (static_cast<uint32_t>(row & 96) << 16) + c0;
+      tc::ld_32x32b_x16(at, r);
       tc::wait_ld();
+      // (kb1 - kb0) / each of them have been written to, rounded up
+      for (int u = 1; u * each < kb1 - kb0; ++u) {
+        uint32_t more[16];
+        tc::ld_32x32b_x16(at + u * g.n, more);
+        tc::wait_ld();
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          r[c] = __float_as_uint(__uint_as_float(r[c]) + __uint_as_float(more[c]));
+      }
       if (g.split > 1) {
 #pragma unroll
         for (int c = 0; c < 16; ++c) mine[(c0 + c) * 128] = __uint_as_float(r[c]);
@@ -426,7 +448,10 @@ __device__ __forceinline__ void tile_at(int t, int tiles_w, int tiles_t, int &tw
 // loading its 128 weight rows and half of the token rows.  Up to n = 224 TMEM
 // holds two accumulators beside the scales, so a tile's MMAs run while the
 // last one is stored.
+// kSums (fp32 C, n <= 224): each kSumBlocks K blocks of a tile go to the next of
+// the two accumulators, and the warps that read them keep the sum.
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-11 accumulators
+template <bool kSums>
 __global__ void __launch_bounds__(kPairThreads, 1)
     k_gemm_pair(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t,
                 const Args g) {
@@ -517,11 +542,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       uint32_t ph = 0;
       unsigned i = 0, piece = 0;  // batches of four K blocks and of sixteen, over all tiles
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step, ++j) {
-        const int a = j % bufs;
-        if (!wait.of_pair(&tempty[a], (static_cast<uint32_t>(j / bufs) & 1) ^ 1)) break;
-        const uint32_t d = tmem + a * n;
+      for (int t = first; t < tiles && ok; t += step) {
+        int a = 0, from = 0;  // the accumulator and its first K block
+        uint32_t d = 0;
         for (int b = 0; 4 * b < g.groups && ok; ++b, ++i) {
+          if (b == 0 || (kSums && 4 * b % kSumBlocks == 0)) {
+            a = j % bufs, from = 4 * b, d = tmem + a * n;
+            ok = wait.of_pair(&tempty[a], (static_cast<uint32_t>(j / bufs) & 1) ^ 1);
+            if (!ok) break;
+            ++j;
+          }
           const int slot = i & 1, buf = piece & 1, kend = min(g.groups, 4 * b + 4);
           // the MMAs of the batch before the last have read this slot's scales
           if (((b & 3) == 0 && !wait.of_pair(&sfull[buf], (piece >> 1) & 1)) ||
@@ -551,7 +581,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 tc::mma_block_scaled<2>(d, dw + 2 * k, dt + 2 * k, idesc, sf_w, sf_t,
-                                        (kb | k) != 0 ? 1u : 0u);
+                                        (kb != from || k != 0) ? 1u : 0u);
               tc::commit_pair(dev::smem_addr(&empty[s]));
             }
             __syncwarp();
@@ -561,13 +591,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (dev::elect_one()) {
             tc::commit<2>(dev::smem_addr(&bdone[slot]));
             if (last) tc::commit_pair(dev::smem_addr(&sfree[buf]));
+            if (kend == g.groups || (kSums && kend % kSumBlocks == 0))
+              tc::commit_pair(dev::smem_addr(&tfull[a]));
           }
           __syncwarp();
           if (last) ++piece;
         }
-        if (!ok) break;
-        if (dev::elect_one()) tc::commit_pair(dev::smem_addr(&tfull[a]));
-        __syncwarp();
       }
       // every MMA issued above is complete once `done` flips
       if (dev::elect_one()) tc::commit<2>(dev::smem_addr(&done));
@@ -600,25 +629,61 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp >= 4) {
     const int q = warp & 3, h = (warp - 4) >> 2, chunks = n / 16;
+    const auto hand_back = [&](int a) {
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive_cluster(tc::map_to_cta(dev::smem_addr(&tempty[a]), 0));
+    };
     int j = 0;
-    for (int t = first; t < tiles; t += step, ++j) {
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
       int tw, tt;
       tile_at(t, tiles_w, tiles_t, tw, tt);
-      const int a = j % bufs;
-      if (!wait(&tfull[a], static_cast<uint32_t>(j / bufs) & 1)) break;
-      tc::fence_after_sync();
       const int w = tw * 256 + rank * 128 + q * 32 + lane;
-      const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + a * n;
-      for (int c = h; c < chunks; c += 2) {
-        uint32_t r[16];
-        tc::ld_32x32b_x16(at + 16 * c, r);
-        tc::wait_ld();
-        if (c + 2 >= chunks) {  // read to the end: hand it back, then store
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) dev::mbar_arrive_cluster(tc::map_to_cta(dev::smem_addr(&tempty[a]), 0));
+      if constexpr (!kSums) {
+        const int a = j % bufs;
+        ok = wait(&tfull[a], static_cast<uint32_t>(j / bufs) & 1);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + a * n;
+        for (int c = h; c < chunks; c += 2) {
+          uint32_t r[16];
+          tc::ld_32x32b_x16(at + 16 * c, r);
+          tc::wait_ld();
+          if (c + 2 >= chunks) hand_back(a);  // read to the end: hand it back, then store
+          store_columns<16>(g, tt * n + 16 * c, w, r);
         }
-        store_columns<16>(g, tt * n + 16 * c, w, r);
+        ++j;
+      } else {
+        // this warp's chunks of 16 columns are h, h + 2, ...: at most 7
+        uint32_t sum[7][16];
+        for (int from = 0; from < g.groups && ok; from += kSumBlocks, ++j) {
+          const int a = j % bufs;
+          ok = wait(&tfull[a], static_cast<uint32_t>(j / bufs) & 1);
+          if (!ok) break;
+          tc::fence_after_sync();
+          const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + a * n + 16 * h;
+#pragma unroll
+          for (int c = 0; c < 7; ++c) {
+            if (h + 2 * c >= chunks) continue;
+            if (from == 0) {
+              tc::ld_32x32b_x16(at + 32 * c, sum[c]);
+              tc::wait_ld();
+            } else {
+              uint32_t r[16];
+              tc::ld_32x32b_x16(at + 32 * c, r);
+              tc::wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                sum[c][e] = __float_as_uint(__uint_as_float(sum[c][e]) + __uint_as_float(r[e]));
+            }
+          }
+          hand_back(a);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 7; ++c)
+          if (h + 2 * c < chunks) store_columns<16>(g, tt * n + 16 * (h + 2 * c), w, sum[c]);
       }
     }
   }
@@ -732,9 +797,11 @@ long long tiles_of(const Args &g, int w, int n) {
 Cut choose_cut(const Args &g, bool skewed) {
   const ClusterRoom room = cluster_room();
   const double read = (static_cast<double>(g.w_rows) + g.t_rows) * g.K / 1e6;
-  Cut best = {256, 0, false};
+  Cut best = {224, 0, false};
   double least = 1e30;
-  for (int n = 32; n <= 256; n += 32) {
+  // sums of several accumulators take two of them at once
+  const bool sums = !g.bf16 && g.groups > kSumBlocks;
+  for (int n = 32; n <= (sums ? 224 : 256); n += 32) {
     const long long waves = (tiles_of(g, 256, n) + current_sm_count() / 2 - 1) /
                             (current_sm_count() / 2);
     const double us = 3.93 + fmax(waves * g.groups * (0.205 + 0.0005 * n) * (skewed ? 1.26 : 1.0),
@@ -773,18 +840,26 @@ Cut choose_cut(const Args &g, bool skewed) {
 
 int launch(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
            cudaStream_t stream) {
-  const Cut cut = choose_cut(g, lda % 128 != 0 || ldb % 128 != 0);
+  Cut cut = choose_cut(g, lda % 128 != 0 || ldb % 128 != 0);
   g.n = cut.n;
   if (cut.split == 0) {
     const long long tiles = tiles_of(g, 256, g.n);
     if (tiles > 0x3fffffffLL) return fail(CMB_ERR_INVALID_ARG, "gemm: too many tiles");
     const int pairs = current_sm_count() / 2;
-    return launch_kernel(k_gemm_pair, A, lda, B, ldb, g, g.n / 2, 2 * (tiles < pairs ? tiles : pairs),
-                         2, kPairThreads, kScaleSlot, kSmemMost, stream);
+    const long long ctas = 2 * (tiles < pairs ? tiles : pairs);
+    auto kernel = !g.bf16 && g.groups > kSumBlocks ? k_gemm_pair<true> : k_gemm_pair<false>;
+    return launch_kernel(kernel, A, lda, B, ldb, g, g.n / 2, ctas, 2, kPairThreads, kScaleSlot,
+                         kSmemMost, stream);
   }
   g.split = cut.split;
+  // one accumulator for each kSumBlocks of a CTA's K blocks where C is fp32, as
+  // far as TMEM goes: half of it, or (one CTA a SM) all
+  const int blocks = (g.groups + g.split - 1) / g.split;
+  g.sums = g.bf16 ? 1 : (blocks + kSumBlocks - 1) / kSumBlocks;
+  if (g.sums > (256 - 16) / g.n) cut.two = false;
+  if (g.sums > (512 - 16) / g.n) g.sums = (512 - 16) / g.n;
   g.tmem_cols = 32;
-  while (g.tmem_cols < g.n + 16) g.tmem_cols *= 2;
+  while (g.tmem_cols < g.sums * g.n + 16) g.tmem_cols *= 2;
   return launch_kernel(k_gemm_split, A, lda, B, ldb, g, g.n, tiles_of(g, 128, g.n) * g.split,
                        g.split, kSplitThreads, kSplitSlot, cut.two ? kSmemHalf : kSmemMost, stream);
 }

@@ -81,10 +81,14 @@ def gemm_bound(ref, mags, k, out):
     """The tensor core adds 32 products at a time to an fp32 accumulator; an
     addition that truncates instead of rounding is off by up to 2 u32, and the
     products' alignment below the largest by as much again: 4 u32 for each
-    32 of K, times the sum of magnitudes (a bound on every partial sum).
-    Rounded once to the output's type."""
-    steps = -(-k // 32) + 1
-    return 4 * U32 * steps * mags + UNIT[out] * np.abs(ref) * (1 + 1e-3) + 1e-300
+    32 of K, times the sum of magnitudes (a bound on every partial sum).  For
+    an fp32 C an accumulator takes 2048 of K, or 2816 where three of 128 tokens
+    share 8192, and the parts are added with a rounding each.  Rounded once to
+    the output's type."""
+    steps = -(-k // 32)
+    if out == "f32" and k <= 8192:
+        steps = min(steps, 2816 // 32) + -(-k // 2048)
+    return 4 * U32 * (steps + 1) * mags + UNIT[out] * np.abs(ref) * (1 + 1e-3) + 1e-300
 
 
 def norm(h, w, eps):

@@ -284,8 +284,32 @@ def test_gemm_large_sampled(cuda, cmb, m, n, k, block_b, out):
     assert (err <= ref.gemm_bound(want, mags, k, out)).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 300, 8192), (100, 512, 6000), (128, 18000, 8192),
+                                   (40, 20000, 4200), (250, 4096, 8192), (2000, 1500, 2049),
+                                   (2100, 2100, 8192), (1500, 4096, 4096), (3000, 3000, 2300)])
+def test_gemm_long_sums_in_fp32(cuda, cmb, m, n, k):
+    """An fp32 C adds accumulators of at most 2048 (2816) of K: all products
+    positive, where truncation would drift one way."""
+    rng = np.random.default_rng(k)
+    a, b = operand(cuda, rng, m, k, 1, wide=0), operand(cuda, rng, n, k, 128, wide=0)
+    for q in (a, b):
+        q[0][:, :k] &= 0x7F
+    qa, qb = a[2] & 0x7F, b[2] & 0x7F
+    c = product(cuda, cmb, a, b, 128, m, n, k, "f32")
+    pick = np.unique(np.concatenate([[0, m - 1], rng.integers(0, m, 40)]))
+    want, mags = ref.gemm(qa[pick], a[3][pick], qb, b[3], 128)
+    err = np.abs(f64(c[cuda.from_numpy(pick).cuda()]) - want)
+    assert (err <= ref.gemm_bound(want, mags, k, "f32")).all()
+    # each of an accumulator's 64 (88) MMAs is off by at most 4 u32 of the sum so
+    # far, as in gemm_bound (2 for the addition and 2 for the alignment of the
+    # products, both downwards, so they do not average out), and the sums so far
+    # of terms that are all positive and alike average half the last one: 88 * 4 *
+    # 1/2.  One accumulator for 8192 would drift by up to 256 * 4 * 1/2.
+    assert np.linalg.norm(err) <= 176 * ref.U32 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 1000, 2064), (48, 4096, 4096), (200, 1000, 3000),
-                                   (3000, 4096, 1024)])
+                                   (3000, 4096, 1024), (3000, 4096, 4500)])
 def test_gemm_same_bits_again(cuda, cmb, m, n, k):
     """No atomics, no order that changes: the same bits from every call, on
     two streams at once too."""
