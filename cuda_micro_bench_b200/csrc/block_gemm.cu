@@ -879,8 +879,8 @@ extern "C" int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_
     return fail(CMB_ERR_INVALID_ARG, "%s: c_type %d is not CMB_BF16 or CMB_F32", fn, c_type);
   if (block_rows_b != 1 && block_rows_b != kBlock)
     return fail(CMB_ERR_INVALID_ARG, "%s: block_rows_b %d not 1 or 128", fn, block_rows_b);
-  if (M < 0 || N < 0 || K < 0 || M > b128::kMostExtent || N > b128::kMostExtent ||
-      K > b128::kMostExtent)
+  // K: a tile's MMAs end well within the 2 s that a wait for them allows
+  if (M < 0 || N < 0 || K < 0 || M > b128::kMostExtent || N > b128::kMostExtent || K > 1 << 28)
     return fail(CMB_ERR_INVALID_ARG, "%s: M %d, N %d, K %d", fn, M, N, K);
   if (reinterpret_cast<uintptr_t>(status) % 4)
     return fail(CMB_ERR_INVALID_ARG, "%s: status is not aligned to its type", fn);

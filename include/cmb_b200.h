@@ -309,10 +309,17 @@ int cmb_quantize_e4m3_block128(const void *src, int src_type, int rows, int cols
  * C.  A linear layer's forward pass has A = activations, B = weights
  * (block_rows_b 128); its input gradient B = the transposed weights; its
  * weight gradient A and B both transposed, block_rows_b 1, K = tokens.
- * M or N = 0 writes nothing; K = 0 writes zeros.  A and B: 16-byte aligned,
- * lda and ldb multiples of 16.  *status (device, may be NULL) is not cleared:
- * it keeps the first CMB_ERR_TIMEOUT of any call since the caller zeroed it,
- * so a program reads it once for many products. */
+ * M or N = 0 writes nothing; K = 0 writes zeros.  K up to 2^28.  A and B:
+ * 16-byte aligned, lda and ldb multiples of 16 (of 128 is faster).  Bytes of A
+ * and B behind a row's K values are not used; scales are read 16 bytes at a
+ * time where their rows start on 16 bytes (a pitch that is a multiple of 16),
+ * so a row's last piece may read behind its last scale, but not use it, up to
+ * the next multiple of 16.  An fp32 C adds accumulators of at most 2048 of K
+ * (2816 for some shapes of up to 128 rows) rounded to nearest, since the
+ * tensor core's own additions truncate.  The die map is not used: the result
+ * does not depend on it.  *status (device, may be NULL) is not cleared: it
+ * keeps the first CMB_ERR_TIMEOUT of any call since the caller zeroed it, so a
+ * program reads it once for many products. */
 int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_t *scale_a, size_t ld_scale_a,
                            const uint8_t *B, size_t ldb, const uint8_t *scale_b, size_t ld_scale_b,
                            int block_rows_b, void *C, size_t ldc, int c_type, int M, int N, int K,
@@ -327,7 +334,9 @@ int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_t *scale_a,
  * elements (bytes for q and scale).  h is written where residual is given
  * (h may be x or residual, element for element); y (the same y rounded to
  * `type`, for a weight gradient), rstd (fp32, one for each row) and the pair
- * q, scale may be NULL.  rows = 0 writes nothing. */
+ * q, scale may be NULL.  But for h, no output may overlap an input or another
+ * output.  rows = 0 writes nothing.  Rows that start on 16 bytes, with cols a
+ * multiple of 8, are fastest. */
 #define CMB_RMSNORM_MAX_COLS 32768
 int cmb_rmsnorm_e4m3_block128(const void *x, size_t ld_x, const void *residual, size_t ld_residual,
                               int type, const void *weight, int weight_type, float eps, int rows,
@@ -344,12 +353,11 @@ size_t cmb_rmsnorm_backward_workspace_bytes(int rows, int cols);
  * h and rstd are the forward pass's (h = x where it had no residual).  dh is
  * the gradient that reaches h past the norm (NULL: none); with a residual,
  * dx is the gradient of x and of the residual alike.  dy, h, dh and dx have
- * `type`; dx may be dy or dh, element for element.  dweight may be NULL, and
- * workspace with it; otherwise workspace is
+ * `type`; dx may be dy or dh, element for element, and overlap nothing else.
+ * dweight may be NULL, and workspace with it; otherwise workspace is
  * cmb_rmsnorm_backward_workspace_bytes(rows, cols) bytes of device memory,
- * 16-byte aligned, that need no initialisation; two calls whose work
- * overlaps on the GPU need separate workspaces.  rows = 0 sets dweight to
- * zeros. */
+ * 16-byte aligned, that need no initialisation; two calls whose work overlaps
+ * on the GPU need separate workspaces.  rows = 0 sets dweight to zeros. */
 int cmb_rmsnorm_backward(const void *dy, size_t ld_dy, const void *h, size_t ld_h, const void *dh,
                          size_t ld_dh, int type, const void *weight, int weight_type,
                          const float *rstd, int rows, int cols, void *dx, size_t ld_dx,

@@ -53,7 +53,7 @@ GEMM = dict(A=P, lda=304, sa=P, ld_sa=3, B=P, ldb=304, sb=P, ld_sb=3, block_rows
 @pytest.mark.parametrize("change,word", [
     (dict(c_type=3), "c_type"), (dict(block_rows_b=2), "block_rows_b"), (dict(M=-1), "M -1"),
     (dict(N=-1), "N -1"), (dict(K=-1), "K -1"), (dict(M=2**31 - 1), "M 2147483647"),
-    (dict(N=2**31 - 1), "N 2147483647"), (dict(K=2**31 - 1), "K 2147483647"), (dict(status=Q), "status"), (dict(C=None), "C is"),
+    (dict(N=2**31 - 1), "N 2147483647"), (dict(K=2**28 + 1, lda=2**29, ldb=2**29, ld_sa=2**22, ld_sb=2**22), "K 268435457"), (dict(status=Q), "status"), (dict(C=None), "C is"),
     (dict(C=Q), "C is"), (dict(C=ctypes.c_void_p(4098), c_type=F32), "C is"),
     (dict(ldc=199), "ldc"), (dict(A=None), "null"), (dict(B=None), "null"), (dict(sa=None), "null"),
     (dict(sb=None), "null"), (dict(A=ctypes.c_void_p(4104)), "16-byte"), (dict(lda=312), "16"),
