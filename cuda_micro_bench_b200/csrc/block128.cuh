@@ -395,9 +395,11 @@ __device__ __forceinline__ void store8_any(T *p, const Raw8<T> &r, int n) {
     store_elements(p, r, 0, n);
     return;
   }
-  const bool joins = lane > 0 && (fulls >> (lane - 1)) & 1, next = lane < 31 && (fulls >> (lane + 1)) & 1;
+  const bool joins = lane > 0 && (fulls >> (lane - 1)) & 1;
+  const bool next = lane < 31 && (fulls >> (lane + 1)) & 1;
   uint4 *piece = reinterpret_cast<uint4 *>(reinterpret_cast<uintptr_t>(p) - m);
-  const int head = static_cast<int>((16 - m) / sizeof(T)), tail = 8 - static_cast<int>(m / sizeof(T));
+  const int head = static_cast<int>((16 - m) / sizeof(T));
+  const int tail = 8 - static_cast<int>(m / sizeof(T));
   if (joins) piece[0] = make_uint4(out[0], out[1], out[2], out[3]);
   else store_elements(p, r, 0, head);
   if constexpr (N == 8) piece[1] = make_uint4(out[4], out[5], out[6], out[7]);

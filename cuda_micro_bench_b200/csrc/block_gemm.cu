@@ -56,7 +56,7 @@ struct Args {
   void *C;
   int w_rows, t_rows, K, groups;
   int w_shift;               // 7 where B has blocks of 128 x 128, else 0
-  bool w_vec, t_vec;     // scale rows can be read 16 bytes at a time
+  bool w_vec, t_vec;         // scale rows can be read 16 bytes at a time
   bool bf16;                 // C's type
   int n;                     // token rows of an MMA
   int stages;
@@ -225,6 +225,9 @@ __device__ __forceinline__ void store_c(const Args &g, int t, int w, float v) {
 // One CTA for each part of the K of a tile of 128 weight rows x n token rows;
 // the `split` CTAs of a tile are one cluster and add their parts, in order,
 // through distributed shared memory.
+// Bound by reading the weights: 1 x 8192 x 8192 takes 13.8 us (67 MB, 10.2 us at
+// the copy rate; 2-3 us of it are the launch and the pipe's start and end), 48 x
+// 4096 x 8192 10.7 us (34 MB, 5.2 us).
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-7 accumulator
 __global__ void __launch_bounds__(kSplitThreads, 2)
     k_gemm_split(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t,
@@ -448,6 +451,11 @@ __device__ __forceinline__ void tile_at(int t, int tiles_w, int tiles_t, int &tw
 // loading its 128 weight rows and half of the token rows.  Up to n = 224 TMEM
 // holds two accumulators beside the scales, so a tile's MMAs run while the
 // last one is stored.
+// Bound by the tensor core and, in a long run, by its power: 8192 x 8192 x 8192
+// takes 382-388 us alone (2.8-2.9 PFLOP/s, the pipe 91 % busy) and 440-470 us
+// back to back, when the SM clock falls from 1.4 to 1.1-1.3 GHz.  L2 hands
+// the SMs 4.9 GB meanwhile.  Wider tiles (256 x 448 in two parts of TMEM, 256 x
+// 480) read less but store with no MMAs beside: 395 and 400 us.
 // kSums (fp32 C, n <= 224): each kSumBlocks K blocks of a tile go to the next of
 // the two accumulators, and the warps that read them keep the sum.
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-11 accumulators
@@ -700,8 +708,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // ------------------------------------------------------------- launches
 
 int launch_kernel(void (*kernel)(CUtensorMap, CUtensorMap, Args), const uint8_t *A, size_t lda,
-                const uint8_t *B, size_t ldb, Args g, int t_box, long long ctas, int cluster,
-                int threads, int slot_bytes, size_t smem_most, cudaStream_t stream) {
+                  const uint8_t *B, size_t ldb, Args g, int t_box, long long ctas, int cluster,
+                  int threads, int slot_bytes, size_t smem_most, cudaStream_t stream) {
   const int stage_bytes = kWBytes + t_box * 128;
   g.stages = static_cast<int>((smem_most - 1024 - 8 * slot_bytes) / stage_bytes);
   if (g.stages > kMaxStages) g.stages = kMaxStages;
@@ -789,9 +797,9 @@ long long tiles_of(const Args &g, int w, int n) {
 // two CTAs share, or a pair, is bound by the bytes that reach it (~0.13 us +
 // 0.7 ns a token; 0.21 us + 0.5 ns; more where rows do not start on 128 bytes,
 // `skewed`, and each 128 bytes of a row lie in two lines); all of it by
-// reading the operands once (5.6 GB/ms).  What a cut adds: parts to sum (0.28 us a doubling + 20 ns a
-// token), columns to store, a wave that starts over.  Some of what it weighs
-// (us): 1 x 8192 x 8192 split 1/2/4: 19.5/14.3/13.7, pairs 20.4; 256 x 8192 x
+// reading the operands once (5.6 GB/ms).  What a cut adds: parts to sum (0.28 us
+// a doubling + 20 ns a token), columns to store, a wave that starts over.  Some
+// of what it weighs (us): 1 x 8192 x 8192 split 1/2/4: 19.5/14.3/13.7, pairs 20.4; 256 x 8192 x
 // 8192 split 1 at n 128: 21.4, pairs 22.4; 1000 x 4600 x 2064 split 16.9, pairs
 // at n 128/224/256: 17.3/20.3/13.3.
 Cut choose_cut(const Args &g, bool skewed) {

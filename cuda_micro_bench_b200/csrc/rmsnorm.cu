@@ -29,7 +29,7 @@ using b128::Raw8;
 
 constexpr int kMaxParts = 1024;  // CTAs, each with a row of partial weight gradients
 // Rows in the ring.  Two leave room for two CTAs of a wide row on a SM, which
-// counts for more than depth: the backward pass of 8192 x 8192 bf16 takes 90 us
+// counts for more than depth: the backward pass of 8192 x 8192 bf16 took 90 us
 // with two, 108 with three or four (one CTA a SM); the norm 81, 80 and 102.
 constexpr int kStages = 2;
 
@@ -192,6 +192,9 @@ __device__ __forceinline__ void store_quantized(const NormArgs &a, int row, int 
   }
 }
 
+// 8192 x 8192 bf16 with a residual and e4m3 out: 75 us for 470 MB, 0.95 of the
+// copy rate.  Without a residual (202 MB) 60 us: the instructions' issue bounds it
+// then, 376 a warp for 512 values.
 template <typename T, typename W, int NV, int kWay>
 __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
   __shared__ float part[2][32];
@@ -275,7 +278,8 @@ struct NormBackArgs {
 
 // Both passes over a row read it from where it lies, the ring's shared memory
 // or global memory, so a thread holds no more of it than a chunk; the weight
-// gradient of its columns stays in registers from row to row.
+// gradient of its columns stays in registers from row to row.  8192 x 8192 bf16
+// with dh: 87 us with the sum below for 537 MB, 0.93 of the copy rate.
 template <typename T, typename W, int NV, int kWay>
 __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) {
   __shared__ float part[2][32];
@@ -379,7 +383,10 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
 }
 
 // dweight[c] = sum of the partial rows: 32 columns a CTA, 32 threads take
-// every 32nd row each, in order, and their sums are added in a tree.
+// every 32nd row each, in order, and their sums are added in a tree.  Latency
+// bound: 334 rows of 4600 columns add 4.7 us to the backward pass (6 MB, from L2);
+// 16 or 8 columns a CTA, 16-byte loads, fewer threads with up to 16 loads each in
+// flight: 4.0-9 us there, none ahead at 8192 columns.
 __global__ void __launch_bounds__(1024) k_sum_parts(const float *__restrict__ parts, size_t ld,
                                                     int n, int cols, float *__restrict__ out) {
   __shared__ float sums[32][33];
