@@ -87,7 +87,9 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
 // zeros), K blocks behind the last anything, which no MMA reads.  32 lanes read
 // 32 rows, so each load is 32 sectors: one for 16 K blocks, all in flight at
 // once.  With a word for 4 K blocks and load the gather, not the tensor core,
-// set the pace (1.0 us a K block of the 480-token tile).
+// set the pace (1.0 us a K block of the 480-token tile).  Plain loads: the kernel
+// may have started before the one that writes the scales ended, which loads
+// through the read-only path do not allow for.
 template <int U>
 __device__ __forceinline__ void scale_pieces(uint4 (&v)[4 * U], const uint8_t *scale, size_t ld,
                                              int row, int rows, int shift, int s, int groups,
@@ -98,7 +100,7 @@ __device__ __forceinline__ void scale_pieces(uint4 (&v)[4 * U], const uint8_t *s
     p[c] = scale + static_cast<size_t>(min(row + 32 * c, rows - 1) >> shift) * ld + 16 * s;
   if (vec) {
 #pragma unroll
-    for (int c = 0; c < 4 * U; ++c) v[c] = __ldg(reinterpret_cast<const uint4 *>(p[c]));
+    for (int c = 0; c < 4 * U; ++c) v[c] = *reinterpret_cast<const uint4 *>(p[c]);
   } else {
     const int last = groups - 1 - 16 * s;
 #pragma unroll
@@ -107,7 +109,7 @@ __device__ __forceinline__ void scale_pieces(uint4 (&v)[4 * U], const uint8_t *s
     for (int i = 0; i <= min(last, 15); ++i) {
       uint32_t byte[4 * U];
 #pragma unroll
-      for (int c = 0; c < 4 * U; ++c) byte[c] = __ldg(p[c] + i);
+      for (int c = 0; c < 4 * U; ++c) byte[c] = p[c][i];
       const int word = i >> 2, at = 8 * (i & 3);
 #pragma unroll
       for (int c = 0; c < 4 * U; ++c) {

@@ -387,8 +387,8 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
 // bound: 334 rows of 4600 columns add 4.7 us to the backward pass (6 MB, from L2);
 // 16 or 8 columns a CTA, 16-byte loads, fewer threads with up to 16 loads each in
 // flight: 4.0-9 us there, none ahead at 8192 columns.
-__global__ void __launch_bounds__(1024) k_sum_parts(const float *__restrict__ parts, size_t ld,
-                                                    int n, int cols, float *__restrict__ out) {
+__global__ void __launch_bounds__(1024) k_sum_parts(const float *parts, size_t ld, int n, int cols,
+                                                    float *out) {
   __shared__ float sums[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   dev::grid_dep_wait();
