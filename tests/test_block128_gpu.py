@@ -763,6 +763,118 @@ def test_layer_in_a_graph_and_on_a_stream(cuda, cmb, tokens):
     assert int(L.status.item()) == 0
 
 
+@pytest.mark.parametrize("where", ["x", "r", "both"])
+def test_norm_in_place_where_rows_follow_one_another(cuda, cmb, where):
+    """More rows than fit at once, so the next row is on its way while h goes
+    over the last; x and the residual may be one tensor."""
+    rng = np.random.default_rng(4)
+    _, x = on_gpu(cuda, activations(rng, 4100, 1544), "bf16")
+    r = x if where == "both" else on_gpu(cuda, rng.normal(size=(4100, 1544)), "bf16")[1]
+    _, w = on_gpu(cuda, np.ones((1, 1544)), "bf16")
+    keep = f64(x), f64(r)
+    out = run_norm(cuda, cmb, x, r, w, "bf16", "bf16", 1e-5, in_place="r" if where == "r" else "x")
+    check_norm(out, *keep, f64(w)[0], "bf16", np.float32(1e-5))
+
+
+@pytest.mark.parametrize("where", ["dy", "dh"])
+def test_norm_backward_in_place_where_rows_follow_one_another(cuda, cmb, where):
+    rng = np.random.default_rng(5)
+    dy, h, dh, w, rstd = backward_inputs(cuda, rng, 4100, 1544, "bf16", "bf16")
+    keep = [f64(t) for t in (dy, h, dh)]
+    dx, grad = run_backward(cuda, cmb, dy, h, dh, w, rstd, "bf16", "bf16",
+                            dx={"dy": dy, "dh": dh}[where])
+    check_backward(dx, grad, *keep, f64(w)[0], f64(rstd), "bf16")
+
+
+@pytest.mark.parametrize("m,k", [(20, 400), (700, 1000)])
+def test_gemm_of_a_matrix_with_itself(cuda, cmb, m, k):
+    rng = np.random.default_rng(m)
+    a = operand(cuda, rng, m, k, 1)
+    c = f64(product(cuda, cmb, a, a, 1, m, m, k, "f32"))
+    want, mags = ref.gemm(a[2], a[3], a[2], a[3], 1)
+    assert (np.abs(c - want) <= ref.gemm_bound(want, mags, k, "f32")).all()
+
+
+def test_products_of_every_kind_on_four_streams(cuda, cmb):
+    """Few tokens (clusters that split K), many (pairs), and the per-tensor
+    product share the GPU and its tensor memory."""
+    rng = np.random.default_rng(6)
+    shapes = [(4, 1024, 4096), (700, 2048, 1024), (100, 3000, 2048)]
+    sets = [(operand(cuda, rng, m, k, 1), operand(cuda, rng, n, k, 128)) for m, n, k in shapes]
+    alone = [product(cuda, cmb, a, b, 128, m, n, k, "bf16").clone()
+             for (a, b), (m, n, k) in zip(sets, shapes)]
+    streams = [cuda.cuda.Stream() for _ in shapes]
+    outs = [cuda.full((6, m, n), 7.0, dtype=cuda.bfloat16, device="cuda") for m, n, _ in shapes]
+    size = 1024
+    ab = cuda.randint(0, 120, (2, size, size), dtype=cuda.uint8, device="cuda")
+    scale = cuda.ones(2, device="cuda")
+    per_tensor = cuda.full((6, size, size), 7.0, device="cuda")
+    st = cuda.zeros(1, dtype=cuda.int32, device="cuda")
+    other = cuda.cuda.Stream()
+    cuda.cuda.synchronize()
+    for i in range(6):
+        for (a, b), (m, n, k), s, out in zip(sets, shapes, streams, outs):
+            cmb.check("cmb_gemm_e4m3_block128", addr(a[0]), a[0].shape[1], addr(a[1]),
+                      a[1].shape[1], addr(b[0]), b[0].shape[1], addr(b[1]), b[1].shape[1], 128,
+                      addr(out[i]), n, BF16, m, n, k, addr(st), ctypes.c_void_p(s.cuda_stream))
+        cmb.check("cmb_gemm_e4m3", addr(ab[0]), addr(ab[1]), addr(per_tensor[i]), size, size,
+                  size, addr(scale), addr(scale), 2, addr(st), ctypes.c_void_p(other.cuda_stream))
+    cuda.cuda.synchronize()
+    assert int(st.item()) == 0
+    for want, out in zip(alone, outs):
+        assert all(cuda.equal(want, c) for c in out)
+    assert all(cuda.equal(per_tensor[0], c) for c in per_tensor)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 512, 1024), (900, 1024, 1024)])
+def test_captured_calls_share_their_buffers(cuda, cmb, m, n, k):
+    """One graph in which the same operand buffers and the same workspace are
+    filled again for each of eight products and gradients: each kernel may
+    start before the last one's end, none may read or write too soon."""
+    rng = np.random.default_rng(8)
+    xs = [on_gpu(cuda, activations(rng, m, k), "bf16")[1] for _ in range(8)]
+    b = operand(cuda, rng, n, k, 128)
+    q, s = (cuda.zeros(m, c, dtype=cuda.uint8, device="cuda") for c in (k, up(k // 128, 16)))
+    w = on_gpu(cuda, np.ones((1, k)), "bf16")[1]
+    rstd = cuda.ones(m, device="cuda")
+    bytes_ = cmb.lib.cmb_rmsnorm_backward_workspace_bytes(m, k)
+    room = cuda.empty(bytes_ // 4, device="cuda")
+    st = cuda.zeros(1, dtype=cuda.int32, device="cuda")
+
+    def steps(wait):
+        outs = []
+        for x in xs:
+            c = cuda.empty(m, n, device="cuda")
+            dx = cuda.empty(m, k, dtype=cuda.bfloat16, device="cuda")
+            dw = cuda.empty(k, device="cuda")
+            room.fill_(float("nan"))
+            cmb.check("cmb_quantize_e4m3_block128", addr(x), BF16, m, k, k, 1, addr(q), k, addr(s),
+                      s.shape[1], None, 0, None, 0, stream_handle(cuda))
+            wait()
+            cmb.check("cmb_gemm_e4m3_block128", addr(q), k, addr(s), s.shape[1], addr(b[0]),
+                      b[0].shape[1], addr(b[1]), b[1].shape[1], 128, addr(c), n, F32, m, n, k,
+                      addr(st), stream_handle(cuda))
+            wait()
+            cmb.check("cmb_rmsnorm_backward", addr(x), k, addr(x), k, None, 0, BF16, addr(w), BF16,
+                      addr(rstd), m, k, addr(dx), k, addr(dw), addr(room), bytes_,
+                      stream_handle(cuda))
+            wait()
+            outs += [c, dx, dw]
+        return outs
+
+    want = steps(cuda.cuda.synchronize)
+    graph, side = cuda.cuda.CUDAGraph(), cuda.cuda.Stream()
+    with cuda.cuda.graph(graph, stream=side):
+        got = steps(lambda: None)
+    for _ in range(3):
+        for t in got:
+            t.fill_(5.0)
+        graph.replay()
+        cuda.cuda.synchronize()
+        assert all(cuda.equal(a, c) for a, c in zip(want, got))
+    assert int(st.item()) == 0
+
+
 def test_command_line_runs_and_checks_the_layer(cuda, tmp_path):
     """`--tensor-ext` times the operators at 8192^3, checks samples of each
     against fp64 and logs what the validator accepts."""
