@@ -875,6 +875,92 @@ def test_captured_calls_share_their_buffers(cuda, cmb, m, n, k):
     assert int(st.item()) == 0
 
 
+# --------------------------------------------- offsets that need more than 32 bits
+
+
+def far_rows(cuda, rows, cols, pitch, dtype, fill):
+    """rows x cols with `pitch` elements from row to row, of which only the
+    values and the one behind each row are written."""
+    assert (rows - 1) * pitch > 2 ** 32
+    v = cuda.empty(rows * pitch, dtype=dtype, device="cuda").view(rows, pitch)
+    v[:, :cols + 1] = fill
+    return v
+
+
+@pytest.fixture
+def room(cuda):
+    cuda.cuda.empty_cache()
+    if cuda.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free device memory")
+    yield
+    cuda.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m", [7, 300])
+def test_gemm_far_offsets(cuda, cmb, room, m):
+    n, k, pitch = 200, 300, up(5 * 2 ** 30 // m, 16)
+    rng = np.random.default_rng(m)
+    a, b = operand(cuda, rng, m, k, 1), operand(cuda, rng, n, k, 128)
+    q, s = (far_rows(cuda, m, w, pitch, cuda.uint8, 0x7F) for w in (k, 3))
+    q[:, :k], s[:, :3] = a[0][:, :k], a[1][:, :3]
+    c = far_rows(cuda, m, n, pitch, cuda.bfloat16, 55.0)
+    cmb.check("cmb_gemm_e4m3_block128", addr(q), pitch, addr(s), pitch, addr(b[0]), b[0].shape[1],
+              addr(b[1]), b[1].shape[1], 128, addr(c), pitch, BF16, m, n, k, None,
+              stream_handle(cuda))
+    want, mags = ref.gemm(a[2], a[3], b[2], b[3], 128)
+    err, room_ = np.abs(f64(c[:, :n]) - want), ref.gemm_bound(want, mags, k, "bf16")
+    assert (err <= room_).all() and (c[:, n] == 55.0).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 300), (5000, 256)])
+def test_norm_and_gradient_far_offsets(cuda, cmb, room, rows, cols):
+    pitch = up(9 * 2 ** 29 // rows, 16)
+    rng = np.random.default_rng(rows)
+    x, dy = (far_rows(cuda, rows, cols, pitch, cuda.bfloat16, 55.0) for _ in range(2))
+    q = far_rows(cuda, rows, cols, pitch, cuda.uint8, FILL)
+    x[:, :cols] = cuda.from_numpy(activations(rng, rows, cols))
+    dy[:, :cols] = cuda.from_numpy(rng.normal(size=(rows, cols)))
+    r, w = (on_gpu(cuda, rng.normal(size=(h, cols)), "bf16")[1] for h in (rows, 1))
+    s = bytes_buffer(cuda, rows, 3)[1]
+    rstd = cuda.empty(rows, device="cuda")
+    keep = f64(x[:, :cols]), f64(r), f64(dy[:, :cols])
+    cmb.check("cmb_rmsnorm_e4m3_block128", addr(x), pitch, addr(r), cols, BF16, addr(w), BF16,
+              ctypes.c_float(1e-5), rows, cols, addr(x), pitch, None, 0, addr(q), pitch, addr(s), 3,
+              addr(rstd), stream_handle(cuda))
+    out = dict(h=x[:, :cols], q=q[:, :cols], s=s[:, :up(cols, 128) // 128], rstd=rstd)
+    check_norm(out, keep[0], keep[1], f64(w)[0], "bf16", np.float32(1e-5))
+    assert (x[:, cols] == 55.0).all() and (q[:, cols] == FILL).all()
+    h = f64(x[:, :cols])
+    grad = cuda.empty(cols, device="cuda")
+    n = cmb.lib.cmb_rmsnorm_backward_workspace_bytes(rows, cols)
+    space = cuda.empty(n, dtype=cuda.uint8, device="cuda")
+    cmb.check("cmb_rmsnorm_backward", addr(dy), pitch, addr(x), pitch, None, 0, BF16, addr(w), BF16,
+              addr(rstd), rows, cols, addr(dy), pitch, addr(grad), addr(space), n,
+              stream_handle(cuda))
+    check_backward(dy[:, :cols], grad, keep[2], h, None, f64(w)[0], f64(rstd), "bf16")
+    assert (dy[:, cols] == 55.0).all()
+
+
+def test_quantize_far_offsets(cuda, cmb, room):
+    rows, cols = 1000, 260
+    src_pitch, pitch_t = up(9 * 2 ** 29 // rows, 16), up(9 * 2 ** 29 // cols, 16)
+    rng = np.random.default_rng(9)
+    x = far_rows(cuda, rows, cols, src_pitch, cuda.bfloat16, 55.0)
+    x[:, :cols] = cuda.from_numpy(activations(rng, rows, cols))
+    q = far_rows(cuda, rows, cols, src_pitch, cuda.uint8, FILL)
+    qt = far_rows(cuda, cols, rows, pitch_t, cuda.uint8, FILL)
+    s, st = bytes_buffer(cuda, rows, 3)[1], bytes_buffer(cuda, cols, 8)[1]
+    cmb.check("cmb_quantize_e4m3_block128", addr(x), BF16, rows, cols, src_pitch, 1, addr(q),
+              src_pitch, addr(s), 3, addr(qt), pitch_t, addr(st), 8, stream_handle(cuda))
+    got = [t.cpu().numpy() for t in (q[:, :cols], s, qt[:, :rows], st)]
+    same_quantized(got, f64(x[:, :cols]), 1)
+    assert (q[:, cols] == FILL).all() and (qt[:, rows] == FILL).all()
+    q[:, :cols], s[:] = FILL, FILL
+    cmb.check("cmb_quantize_e4m3_block128", addr(x), BF16, rows, cols, src_pitch, 1, addr(q),
+              src_pitch, addr(s), 3, None, 0, None, 0, stream_handle(cuda))
+    same_quantized([q[:, :cols].cpu().numpy(), s.cpu().numpy(), None, None], f64(x[:, :cols]), 1)
+
+
 def test_command_line_runs_and_checks_the_layer(cuda, tmp_path):
     """`--tensor-ext` times the operators at 8192^3, checks samples of each
     against fp64 and logs what the validator accepts."""
