@@ -800,10 +800,11 @@ long long tiles_of(const Args &g, int w, int n) {
 // 0.7 ns a token; 0.21 us + 0.5 ns; more where rows do not start on 128 bytes,
 // `skewed`, and each 128 bytes of a row lie in two lines); all of it by
 // reading the operands once (5.6 GB/ms).  What a cut adds: parts to sum (0.28 us
-// a doubling + 20 ns a token), columns to store, a wave that starts over.  Some
-// of what it weighs (us): 1 x 8192 x 8192 split 1/2/4: 19.5/14.3/13.7, pairs 20.4; 256 x 8192 x
-// 8192 split 1 at n 128: 21.4, pairs 22.4; 1000 x 4600 x 2064 split 16.9, pairs
-// at n 128/224/256: 17.3/20.3/13.3.
+// a doubling + 20 ns a token), columns to store, which a short K does not
+// hide, a wave that starts over.  Some of what it weighs (us): 1 x 8192 x 8192
+// split 1/2/4: 19.5/14.3/13.7, pairs 20.4; 256 x 8192 x 8192 split 1 at n 128:
+// 21.4, pairs 22.4; 1000 x 4600 x 2064 split 16.9, pairs at n 128/224/256:
+// 17.3/20.3/13.3.
 Cut choose_cut(const Args &g, bool skewed) {
   const ClusterRoom room = cluster_room();
   const double read = (static_cast<double>(g.w_rows) + g.t_rows) * g.K / 1e6;
@@ -814,7 +815,9 @@ Cut choose_cut(const Args &g, bool skewed) {
   for (int n = 32; n <= (sums ? 224 : 256); n += 32) {
     const long long waves = (tiles_of(g, 256, n) + current_sm_count() / 2 - 1) /
                             (current_sm_count() / 2);
-    const double us = 3.93 + fmax(waves * g.groups * (0.205 + 0.0005 * n) * (skewed ? 1.26 : 1.0),
+    const double sum = g.groups * (0.205 + 0.0005 * n) * (skewed ? 1.26 : 1.0);
+    const double store = g.bf16 ? 0.8 + 0.0075 * n : 0.52 + 0.0125 * n;
+    const double us = 3.93 + fmax(waves * sum + (waves - 1) * fmax(0.0, store - 0.6 * sum),
                                   0.194 * read) +
                       0.007 * n + (2 * n > kScaleCol ? 3.0 * (waves - 1) : 0.0);
     if (us < least) least = us, best = {n, 0, false};
