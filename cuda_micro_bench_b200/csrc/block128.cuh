@@ -361,6 +361,62 @@ __device__ __forceinline__ Raw8<T> load8_any(const T *p, int n, const Bounds &in
   return r;
 }
 
+// load8_any in two steps with no branch in the first, so that many fetches are on
+// their way before the first is cut to size: the aligned pieces around 8 elements.
+template <typename T>
+struct Cut8 {
+  static constexpr int kWords = sizeof(T) * 2, kPieces = kWords / 4 + 1;
+  uint4 piece[kPieces];
+  bool edge;  // a piece goes past the matrix
+};
+
+template <typename T>
+__device__ __forceinline__ Cut8<T> fetch8(const T *p, int n, const Bounds &in) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t(15);
+  const uintptr_t end = at + max(0, min(n, 8)) * sizeof(T);
+  Cut8<T> c;
+  c.edge = false;
+#pragma unroll
+  for (int k = 0; k < Cut8<T>::kPieces; ++k) {
+    const uintptr_t piece = first + 16 * k;
+    const bool wanted = piece < end && n > 0;
+    const bool there = piece >= in.begin && piece + 16 <= in.end;
+    c.piece[k] = make_uint4(0, 0, 0, 0);
+    if (wanted && there) c.piece[k] = *reinterpret_cast<const uint4 *>(piece);
+    c.edge |= wanted && !there;
+  }
+  return c;
+}
+
+// Elements [0, n) of the 8 at p, zeros behind them.
+template <typename T>
+__device__ __forceinline__ Raw8<T> cut8(Cut8<T> &c, const T *p, int n) {
+  constexpr int N = Cut8<T>::kWords;
+  Raw8<T> r;
+  if (c.edge) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.0f;
+    pack(v, r);
+    return r;
+  }
+  uint32_t in[N + 4], w[N];
+#pragma unroll
+  for (int k = 0; k < Cut8<T>::kPieces; ++k) {
+    const uint4 v = c.piece[k];
+    in[4 * k] = v.x, in[4 * k + 1] = v.y, in[4 * k + 2] = v.z, in[4 * k + 3] = v.w;
+  }
+  from_byte<N>(in, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15), w);
+  if (n < 8) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int left = n * static_cast<int>(sizeof(T)) - 4 * i;  // bytes of this word
+      if (left < 4) w[i] = left > 0 ? w[i] & ((1u << (8 * left)) - 1) : 0u;
+    }
+  }
+  return from_words<T>(w);
+}
+
 template <typename T>
 __device__ __forceinline__ void store_elements(T *p, const Raw8<T> &r, int from, int to) {
   float v[8];

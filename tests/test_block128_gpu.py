@@ -115,6 +115,20 @@ def test_quantize_strides_and_alignment(cuda, cmb, kind, block, pitch, pad, offs
     same_quantized(quantize(cuda, cmb, view, kind, block, "both", pad, offset), f64(view), block)
 
 
+@pytest.mark.parametrize("which", ["rows", "both"])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("cols,pad,offset", [(1304, 0, 0), (1304, 8, 0), (1304, 1, 0), (1301, 0, 3)])
+def test_quantize_many_tiles(cuda, cmb, kind, cols, pad, offset, which):
+    """More tiles than SMs, whose edges and odd rows are read ahead of one
+    another, with values that are not finite in some."""
+    rng = np.random.default_rng(cols + pad)
+    x = activations(rng, 2500, cols)
+    x[rng.integers(0, 2500, 9), rng.integers(0, cols, 9)] = [np.inf, -np.inf, np.nan] * 3
+    x[0, 0] = x[-1, -1] = np.inf
+    _, view = on_gpu(cuda, x, kind, offset=offset)
+    same_quantized(quantize(cuda, cmb, view, kind, 1, which, pad), f64(view), 1)
+
+
 @pytest.mark.parametrize("block", [1, 128])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_quantize_borders(cuda, cmb, kind, block):
