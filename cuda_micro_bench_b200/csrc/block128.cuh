@@ -328,22 +328,22 @@ struct Bounds {
   }
 };
 
-// Elements [0, n) of the 8 at p, zeros behind them.
+// Elements [0, n) of the 8 at byte m of the aligned 16-byte pieces around them,
+// zeros behind them.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8_any(const T *p, int n, const Bounds &in) {
-  constexpr int N = sizeof(T) * 2;  // words
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p), piece = at & ~uintptr_t(15);
-  uint32_t w[N];
-  if (n <= 0) return Raw8<T>{};
-  if (at == piece && n >= 8) return load8(p);
-  if (piece >= in.begin && piece + 4 * N + 16 <= in.end) {
-    uint32_t c[N + 4];
+struct Pieces8 {
+  static constexpr int kWords = sizeof(T) * 2, kPieces = kWords / 4 + 1;
+  uint4 piece[kPieces];
+
+  __device__ __forceinline__ Raw8<T> cut(uint32_t m, int n) const {
+    constexpr int N = kWords;
+    uint32_t in[N + 4], w[N];
 #pragma unroll
-    for (int i = 0; i < N / 4 + 1; ++i) {
-      const uint4 v = reinterpret_cast<const uint4 *>(piece)[i];
-      c[4 * i] = v.x, c[4 * i + 1] = v.y, c[4 * i + 2] = v.z, c[4 * i + 3] = v.w;
+    for (int k = 0; k < kPieces; ++k) {
+      const uint4 v = piece[k];
+      in[4 * k] = v.x, in[4 * k + 1] = v.y, in[4 * k + 2] = v.z, in[4 * k + 3] = v.w;
     }
-    from_byte<N>(c, static_cast<uint32_t>(at - piece), w);
+    from_byte<N>(in, m, w);
     if (n < 8) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -353,6 +353,11 @@ __device__ __forceinline__ Raw8<T> load8_any(const T *p, int n, const Bounds &in
     }
     return from_words<T>(w);
   }
+};
+
+// The same one element at a time.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_elements(const T *p, int n) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.0f;
@@ -361,61 +366,48 @@ __device__ __forceinline__ Raw8<T> load8_any(const T *p, int n, const Bounds &in
   return r;
 }
 
-// load8_any in two steps with no branch in the first, so that many fetches are on
-// their way before the first is cut to size: the aligned pieces around 8 elements.
-template <typename T>
-struct Cut8 {
-  static constexpr int kWords = sizeof(T) * 2, kPieces = kWords / 4 + 1;
-  uint4 piece[kPieces];
-  bool edge;  // a piece goes past the matrix
-};
-
-template <typename T>
-__device__ __forceinline__ Cut8<T> fetch8(const T *p, int n, const Bounds &in) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t(15);
-  const uintptr_t end = at + max(0, min(n, 8)) * sizeof(T);
-  Cut8<T> c;
-  c.edge = false;
-#pragma unroll
-  for (int k = 0; k < Cut8<T>::kPieces; ++k) {
-    const uintptr_t piece = first + 16 * k;
-    const bool wanted = piece < end && n > 0;
-    const bool there = piece >= in.begin && piece + 16 <= in.end;
-    c.piece[k] = make_uint4(0, 0, 0, 0);
-    if (wanted && there) c.piece[k] = *reinterpret_cast<const uint4 *>(piece);
-    c.edge |= wanted && !there;
-  }
-  return c;
-}
-
 // Elements [0, n) of the 8 at p, zeros behind them.
 template <typename T>
-__device__ __forceinline__ Raw8<T> cut8(Cut8<T> &c, const T *p, int n) {
-  constexpr int N = Cut8<T>::kWords;
-  Raw8<T> r;
-  if (c.edge) {
-    float v[8];
+__device__ __forceinline__ Raw8<T> load8_any(const T *p, int n, const Bounds &in) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), piece = at & ~uintptr_t(15);
+  if (n <= 0) return Raw8<T>{};
+  if (at == piece && n >= 8) return load8(p);
+  if (piece >= in.begin && piece + 16 * Pieces8<T>::kPieces <= in.end) {
+    Pieces8<T> c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.0f;
-    pack(v, r);
-    return r;
+    for (int k = 0; k < Pieces8<T>::kPieces; ++k)
+      c.piece[k] = reinterpret_cast<const uint4 *>(piece)[k];
+    return c.cut(static_cast<uint32_t>(at - piece), n);
   }
-  uint32_t in[N + 4], w[N];
+  return load_elements(p, n);
+}
+
+// load8_any in two steps with no branch in the first, so that many fetches are on
+// their way before the first is cut to size.
+template <typename T>
+struct Fetch8 {
+  Pieces8<T> pieces;
+  bool edge;  // a piece goes past the matrix
+
+  __device__ __forceinline__ Fetch8(const T *p, int n, const Bounds &in) : edge(false) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), first = at & ~uintptr_t(15);
+    const uintptr_t end = at + min(n, 8) * sizeof(T);
 #pragma unroll
-  for (int k = 0; k < Cut8<T>::kPieces; ++k) {
-    const uint4 v = c.piece[k];
-    in[4 * k] = v.x, in[4 * k + 1] = v.y, in[4 * k + 2] = v.z, in[4 * k + 3] = v.w;
-  }
-  from_byte<N>(in, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15), w);
-  if (n < 8) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int left = n * static_cast<int>(sizeof(T)) - 4 * i;  // bytes of this word
-      if (left < 4) w[i] = left > 0 ? w[i] & ((1u << (8 * left)) - 1) : 0u;
+    for (int k = 0; k < Pieces8<T>::kPieces; ++k) {
+      const uintptr_t piece = first + 16 * k;
+      const bool wanted = n > 0 && piece < end;
+      const bool there = piece >= in.begin && piece + 16 <= in.end;
+      pieces.piece[k] = make_uint4(0, 0, 0, 0);
+      if (wanted && there) pieces.piece[k] = *reinterpret_cast<const uint4 *>(piece);
+      edge |= wanted && !there;
     }
   }
-  return from_words<T>(w);
-}
+  Fetch8() = default;
+  __device__ __forceinline__ Raw8<T> get(const T *p, int n) const {
+    if (edge) return load_elements(p, n);
+    return pieces.cut(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15), n);
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ void store_elements(T *p, const Raw8<T> &r, int from, int to) {

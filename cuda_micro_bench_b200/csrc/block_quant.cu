@@ -302,13 +302,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize_tile(c
       // both ways took 66 us instead of 53
 #pragma unroll
       for (int half = 0; half < 8; half += 4) {
-        b128::Cut8<T> cut[4];
+        b128::Fetch8<T> row[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          cut[i] = b128::fetch8(from + i * a.ld_src, half + i < p.nrow ? p.ncol : 0, in);
+          row[i] = b128::Fetch8<T>(from + i * a.ld_src, half + i < p.nrow ? p.ncol : 0, in);
 #pragma unroll
         for (int i = 0; i < 4; ++i, from += a.ld_src)
-          p.raw[half + i] = b128::cut8(cut[i], from, half + i < p.nrow ? p.ncol : 0);
+          p.raw[half + i] = row[i].get(from, half + i < p.nrow ? p.ncol : 0);
       }
     }
     const bool any = tile_scales<true>(a, p, tile_r, row_in, col_in, sh);
