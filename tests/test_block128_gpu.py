@@ -975,6 +975,42 @@ def test_quantize_far_offsets(cuda, cmb, room):
     same_quantized([q[:, :cols].cpu().numpy(), s.cpu().numpy(), None, None], f64(x[:, :cols]), 1)
 
 
+FIRST_IN_A_GRAPH = """
+import torch
+import cuda_micro_bench_b200 as cmb
+from tests.test_block128_gpu import Layer
+for tokens in (1, 200):
+    L = Layer(torch, cmb, tokens, 640, 500, 1)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        L.forward()
+        L.backward()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = {n: t.clone() for n, t in L.outputs().items()}
+    L.forward()
+    L.backward()
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, got[n]) for n, t in L.outputs().items())
+    assert int(L.status.item()) == 0
+print("same")
+"""
+
+
+def test_first_call_of_a_process_is_captured(cuda):
+    """What the library asks the driver once (addresses, how many clusters fit)
+    may be asked while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], cwd=root,
+                         capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
+
+
 def test_command_line_runs_and_checks_the_layer(cuda, tmp_path):
     """`--tensor-ext` times the operators at 8192^3, checks samples of each
     against fp64 and logs what the validator accepts."""
