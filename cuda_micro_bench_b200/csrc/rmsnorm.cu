@@ -443,12 +443,14 @@ Shape shape_for(int rows, int cols, int nv, size_t row_bytes, bool sums) {
   return s;
 }
 
-constexpr size_t kRingMost = 200 * 1024;
+constexpr size_t kRingMost = 200 * 1024;  // no launch takes more shared memory
 
 template <typename A>
 int launch_rows(void (*kernel)(A), const A &a, const Shape &s, cudaStream_t stream) {
+  // One limit for every launch of the kernel: it is the function's, not the
+  // call's, and another host thread may be between these two lines.
   CMB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(s.smem)));
+                                    static_cast<int>(kRingMost)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(s.grid);
   cfg.blockDim = dim3(s.x, s.y);
