@@ -335,8 +335,9 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
     if constexpr (kWay == kRing)
       if (threadIdx.x == 0 && threadIdx.y == 0 && turn > 0) ring.load(turn - 1 + kStages, a.rows);
     if (!here) continue;
-    // dx = rstd g - h rstd^3 mean(g h) + dh
-    const float minus = -rstd * rstd * (rstd * (sum / static_cast<float>(a.cols)));
+    // dx = rstd (g + h minus) + dh with minus = -rstd^2 mean(g h).  rstd mean(g h) is
+    // of the size of g: rstd^2 alone is past fp32 for rows under 5e-20 (eps 0).
+    const float minus = -rstd * (rstd * (sum / static_cast<float>(a.cols)));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = (i * blockDim.x + threadIdx.x) * 8, n = a.cols - col;
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
       if (a.dh != nullptr)
         b128::unpack(load_chunk<T, kWay>(ring, turn, 2, a.dh, a.ld_dh, row, col, n, in_dh), past);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = fmaf(rstd, g[j], fmaf(u[j], minus, past[j]));
+      for (int j = 0; j < 8; ++j) g[j] = fmaf(rstd, fmaf(u[j], minus, g[j]), past[j]);
       store_chunk<T, kWay>(a.dx, a.ld_dx, row, col, n, b128::packed<T>(g));
     }
   }

@@ -336,8 +336,9 @@ int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_t *scale_a,
  * `type`, for a weight gradient), rstd (fp32, one for each row) and the pair
  * q, scale may be NULL.  But for h, no output may overlap an input or another
  * output.  rows = 0 writes nothing.  Sums are fp32: a row whose squares overflow
- * (values past 1e18 or so) has rstd 0.  Rows that start on 16 bytes, with cols
- * a multiple of 8, are fastest. */
+ * (values past 1e18 or so) has rstd 0; with eps 0, rows under 1e-19 lose bits with
+ * their squares, and one whose squares are all 0 has rstd infinite and NaN in y.
+ * Rows that start on 16 bytes, with cols a multiple of 8, are fastest. */
 #define CMB_RMSNORM_MAX_COLS 32768
 int cmb_rmsnorm_e4m3_block128(const void *x, size_t ld_x, const void *residual, size_t ld_residual,
                               int type, const void *weight, int weight_type, float eps, int rows,

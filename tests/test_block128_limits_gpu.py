@@ -67,3 +67,26 @@ def test_norms_of_different_widths_from_four_threads(cuda, cmb, op):
     cuda.cuda.synchronize()
     assert refused == [0] * 4
     assert all(cuda.equal(out, alone) for _, out, alone, _, _ in jobs)
+
+
+# ------------------------------------------------ rows near the ends of fp32
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(3, 300), (5, 8192), (600, 4096), (900, 1031)])
+def test_gradient_of_rows_whose_rstd_squared_is_past_fp32(cuda, cmb, rows, cols, kind, residual):
+    """Rows of 1e-20 and of 1e15 beside ordinary ones, eps = 0: rstd is 1e20, its
+    square is not a number of fp32, and dx (of 1e20 times dy) is."""
+    rng = np.random.default_rng(cols)
+    size = np.array([1e-20, 1.0, 1e15, 3e-20, 1e-19])[np.arange(rows) % 5][:, None]
+    _, dy = on_gpu(cuda, rng.normal(size=(rows, cols)), kind)
+    _, h = on_gpu(cuda, rng.normal(size=(rows, cols)) * size, kind)
+    dh = on_gpu(cuda, rng.normal(size=(rows, cols)) / size, kind)[1] if residual else None
+    _, w = on_gpu(cuda, 1 + 0.1 * rng.normal(size=(1, cols)), "f32")
+    rstd = (1 / h.double().square().mean(dim=1).sqrt()).float()
+    assert float(rstd.max()) > 2.0 ** 64
+    dx, grad = run_backward(cuda, cmb, dy, h, dh, w, rstd, kind, "f32")
+    assert cuda.isfinite(dx).all()
+    check_backward(dx, grad, f64(dy), f64(h), f64(dh) if residual else None, f64(w)[0], f64(rstd),
+                   kind)
