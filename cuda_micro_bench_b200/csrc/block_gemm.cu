@@ -62,7 +62,7 @@ struct Args {
   int stages;
   int split;                 // CTAs that share a tile's K (k_gemm_split)
   int tmem_cols;             // TMEM columns to allocate (k_gemm_split)
-  int sums;                  // accumulators that share a CTA's K (k_gemm_split)
+  int sums;                  // accumulators in TMEM for a CTA's K (k_gemm_split)
   int *status;
 };
 
@@ -74,7 +74,8 @@ constexpr int kScaleCol = 480;          // TMEM columns of the scales: 2 x 4 and
 constexpr size_t kSmemMost = 227 * 1024 - 1024;  // less what is static
 constexpr size_t kSmemHalf = 112 * 1024;         // two CTAs a SM
 constexpr int kSplitThreads = 256;
-constexpr int kSumBlocks = 16;  // K blocks of an accumulator where C is fp32
+// K blocks of an accumulator where C is fp32: as many as share a fetch of scales
+constexpr int kSumBlocks = 16;
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d) {
@@ -230,8 +231,13 @@ __device__ __forceinline__ void store_c(const Args &g, int t, int w, float v) {
 // Bound by reading the weights: 1 x 8192 x 8192 takes 13.8 us (67 MB, 10.2 us at
 // the copy rate; 2-3 us of it are the launch and the pipe's start and end), 48 x
 // 4096 x 8192 10.7 us (34 MB, 5.2 us).
-//   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-7 accumulator
-__global__ void __launch_bounds__(kSplitThreads, 2)
+// kParts: where TMEM does not hold an accumulator for each kSumBlocks K blocks,
+// two of them take turns, one for each 16 K blocks whose scales come together, and
+// warps 4-7 keep the sum, as in k_gemm_pair<true>.  The sum's 128 registers a thread
+// leave room for one CTA a SM, as so many accumulators do.
+//   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-7 accumulators
+template <bool kParts>
+__global__ void __launch_bounds__(kSplitThreads, kParts ? 1 : 2)
     k_gemm_split(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t,
                  const Args g) {
   extern __shared__ uint8_t smem_raw[];
@@ -239,6 +245,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
                                               ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages];
   __shared__ __align__(8) uint64_t sfull[2], sfree[2], bdone[2], done;
+  __shared__ __align__(8) uint64_t tfull[2], tempty[2];  // kParts
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
 
@@ -260,6 +267,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       dev::mbar_init(dev::smem_addr(&sfull[s]), 1);
       dev::mbar_init(dev::smem_addr(&sfree[s]), 1);
       dev::mbar_init(dev::smem_addr(&bdone[s]), 1);
+      if constexpr (kParts) {
+        dev::mbar_init(dev::smem_addr(&tfull[s]), 1);
+        dev::mbar_init(dev::smem_addr(&tempty[s]), 4);  // warps 4-7
+      }
     }
     dev::mbar_init(dev::smem_addr(&done), 1);
     abort_flag = 0;
@@ -275,7 +286,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = uniform(tmem_holder);
-  const int each = (kb1 - kb0 + g.sums - 1) / g.sums;  // K blocks of an accumulator
+  const int each = (kb1 - kb0 + g.sums - 1) / g.sums;  // K blocks of an accumulator (!kParts)
   const Waiter wait{&abort_flag, g.status};
   dev::grid_dep_wait();
   dev::grid_dep_launch();
@@ -311,6 +322,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     for (int b = kb0 >> 2; b <= (kb1 - 1) >> 2 && ok; ++b, ++i) {
       const int slot = i & 1, piece = (b >> 2) - (kb0 >> 4), buf = piece & 1;
       if ((i == 0 || (b & 3) == 0) && !wait(&sfull[buf], (piece >> 1) & 1)) break;
+      // the part before the last has been read from this part's accumulator
+      if (kParts && (i == 0 || (b & 3) == 0) && !wait(&tempty[buf], ((piece >> 1) & 1) ^ 1)) break;
       // the MMAs of the batch before the last have read this slot's scales
       if (!wait(&bdone[slot], ((i >> 1) & 1) ^ 1)) break;
       tc::fence_after_sync();
@@ -331,8 +344,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         const uint32_t w = dev::smem_addr(ring + (size_t)s * stage_bytes);
         const uint64_t dw = tc::sw128_kmajor_desc(w), dt = tc::sw128_kmajor_desc(w + kWBytes);
         const uint32_t idesc = tc::instr_desc_block_scaled(128, g.n, kb & 3);
-        const uint32_t d = tmem + sum * g.n;
-        const bool first = left == each;  // of its accumulator
+        const uint32_t d = kParts ? tmem + buf * g.n : tmem + sum * g.n;
+        // of its accumulator
+        const bool first = kParts ? kb == kb0 || (kb & 15) == 0 : left == each;
         if (dev::elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -342,11 +356,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         }
         __syncwarp();
         if (++s == g.stages) s = 0, ph ^= 1;
-        if (--left == 0) left = each, ++sum;
+        if (!kParts && --left == 0) left = each, ++sum;
       }
       if (dev::elect_one()) {
         tc::commit<1>(dev::smem_addr(&bdone[slot]));
         if ((b & 3) == 3) tc::commit<1>(dev::smem_addr(&sfree[buf]));
+        if (kParts && ((b & 3) == 3 || end == kb1)) tc::commit<1>(dev::smem_addr(&tfull[buf]));
       }
       __syncwarp();
     }
@@ -370,6 +385,48 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       dev::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) dev::mbar_arrive(dev::smem_addr(&sfull[buf]));
+    }
+  } else if (kParts && warp >= 4) {
+    const int row = (warp & 3) * 32 + lane;
+    uint32_t sum[8][16];  // n is at most 128
+    bool ok = true;
+    const int pieces = ((kb1 - 1) >> 4) - (kb0 >> 4) + 1;
+    for (int j = 0; j < pieces; ++j) {
+      const int a = j & 1;
+      ok = wait(&tfull[a], (j >> 1) & 1);
+      if (!ok) break;
+      tc::fence_after_sync();
+      const uint32_t at = tmem + (static_cast<uint32_t>(row & 96) << 16) + a * g.n;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (16 * c >= g.n) continue;
+        if (j == 0) {
+          tc::ld_32x32b_x16(at + 16 * c, sum[c]);
+          tc::wait_ld();
+        } else {
+          uint32_t r[16];
+          tc::ld_32x32b_x16(at + 16 * c, r);
+          tc::wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            sum[c][e] = __float_as_uint(__uint_as_float(sum[c][e]) + __uint_as_float(r[e]));
+        }
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive(dev::smem_addr(&tempty[a]));
+    }
+    // every load has landed and every MMA has read it: the ring takes the sums
+    float *mine = reinterpret_cast<float *>(ring) + row;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (16 * c >= g.n || !ok) continue;
+      if (g.split > 1) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(16 * c + e) * 128] = __uint_as_float(sum[c][e]);
+      } else {
+        store_columns<16>(g, t0 + 16 * c, w0 + row, sum[c]);
+      }
     }
   } else if (warp >= 4) {
     const bool ok = wait(&done, 0);
@@ -760,7 +817,7 @@ ClusterRoom cluster_room() {
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return room;
   std::lock_guard<std::mutex> lock(mu);
   if (known[device].clusters[0] != 0) return known[device];
-  cudaFuncSetAttribute(k_gemm_split, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaFuncSetAttribute(k_gemm_split<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                        static_cast<int>(kSmemMost));
   for (int i = 0; i < 4; ++i) {
     cudaLaunchConfig_t cfg = {};
@@ -775,7 +832,7 @@ ClusterRoom cluster_room() {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, k_gemm_split, &cfg) == cudaSuccess && n > 0)
+    if (cudaOccupancyMaxActiveClusters(&n, k_gemm_split<false>, &cfg) == cudaSuccess && n > 0)
       room.clusters[i] = n;
   }
   return known[device] = room;
@@ -865,15 +922,16 @@ int launch(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
                          kSmemMost, stream);
   }
   g.split = cut.split;
-  // one accumulator for each kSumBlocks of a CTA's K blocks where C is fp32, as
-  // far as TMEM goes: half of it, or (one CTA a SM) all
+  // one accumulator for each kSumBlocks of a CTA's K blocks where C is fp32: in
+  // half of TMEM or (one CTA a SM) all of it, or two that take turns
   const int blocks = (g.groups + g.split - 1) / g.split;
   g.sums = g.bf16 ? 1 : (blocks + kSumBlocks - 1) / kSumBlocks;
   if (g.sums > (256 - 16) / g.n) cut.two = false;
-  if (g.sums > (512 - 16) / g.n) g.sums = (512 - 16) / g.n;
+  const bool parts = g.sums > (512 - 16) / g.n;
+  if (parts) g.sums = 2;
   g.tmem_cols = 32;
   while (g.tmem_cols < g.sums * g.n + 16) g.tmem_cols *= 2;
-  return launch_kernel(k_gemm_split, A, lda, B, ldb, g, g.n, tiles_of(g, 128, g.n) * g.split,
+  return launch_kernel(parts ? k_gemm_split<true> : k_gemm_split<false>, A, lda, B, ldb, g, g.n, tiles_of(g, 128, g.n) * g.split,
                        g.split, kSplitThreads, kSplitSlot, cut.two ? kSmemHalf : kSmemMost, stream);
 }
 

@@ -90,3 +90,71 @@ def test_gradient_of_rows_whose_rstd_squared_is_past_fp32(cuda, cmb, rows, cols,
     assert cuda.isfinite(dx).all()
     check_backward(dx, grad, f64(dy), f64(h), f64(dh) if residual else None, f64(w)[0], f64(rstd),
                    kind)
+
+
+# ------------------------------------------------------------- long sums
+
+
+def long_operand(cuda, rows, k, block, seed, signed):
+    """Random finite codes made on the GPU, with scales of 1/4 .. 4; NaN codes and
+    scales behind each row."""
+    gen = cuda.Generator(device="cuda").manual_seed(seed)
+    pitch, groups = up(k, 16), up(k, 128) // 128
+    q = cuda.randint(0, 127, (rows, pitch), dtype=cuda.uint8, device="cuda", generator=gen)
+    if signed:
+        q |= cuda.randint(0, 2, (rows, pitch), dtype=cuda.uint8, device="cuda", generator=gen) << 7
+    q[:, k:] = 0x7F
+    s = cuda.full((-(-rows // block), groups + 3), 255, dtype=cuda.uint8, device="cuda")
+    s[:, :groups] = cuda.randint(125, 130, (s.shape[0], groups), dtype=cuda.uint8, device="cuda",
+                                 generator=gen)
+    return q, s
+
+
+def long_values(q, s, rows, k, block):
+    """What those rows stand for, in 64 bits."""
+    groups = up(k, 128) // 128
+    codes = q[rows][:, :k].cpu().numpy()
+    scales = s[rows // block][:, :groups].cpu().numpy()
+    return ref.VALUES[codes] * ref.spread(scales, len(rows), k, 1)
+
+
+def long_product(cuda, cmb, m, n, k, block_b, out, signed):
+    """The product, and its rows and columns that are compared: ends and a few."""
+    a, b = long_operand(cuda, m, k, 1, 1, signed), long_operand(cuda, n, k, block_b, 2, signed)
+    c = cuda.full((m, n), float("nan"), dtype=cuda.bfloat16 if out == "bf16" else cuda.float32,
+                  device="cuda")
+    status = cuda.zeros(1, dtype=cuda.int32, device="cuda")
+    cmb.check("cmb_gemm_e4m3_block128", addr(a[0]), a[0].shape[1], addr(a[1]), a[1].shape[1],
+              addr(b[0]), b[0].shape[1], addr(b[1]), b[1].shape[1], block_b, addr(c), n, CODE[out],
+              m, n, k, addr(status), stream_handle(cuda))
+    assert int(status.item()) == 0 and bool(cuda.isfinite(c).all())
+    rng = np.random.default_rng(k)
+    pick = lambda size, some: np.unique(np.concatenate([[0, size - 1], rng.integers(0, size, some)]))
+    rows, cols = pick(m, 24), pick(n, 40)
+    got = f64(c[cuda.from_numpy(rows).cuda()][:, cuda.from_numpy(cols).cuda()])
+    x = long_values(*a, rows, k, 1)
+    y = long_values(*b, cols, k, block_b)
+    return got, x @ y.T, np.abs(x) @ np.abs(y).T
+
+
+# few tokens and many, one CTA a tile and up to eight, whole and odd sizes
+LONG = [(128, 18944, 16384), (160, 8192, 28672), (128, 9472, 53248), (2048, 2048, 131072),
+        (512, 1000, 100003), (97, 700, 70001), (3, 1030, 2 ** 21 - 77), (16, 256, 2 ** 21),
+        (300, 5000, 30000)]
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+@pytest.mark.parametrize("signed", [False, True])
+def test_gemm_fp32_sums_of_any_length(cuda, cmb, m, n, k, signed):
+    """An fp32 C adds accumulators of 2048 of K.  An accumulator's 64 MMAs are off
+    by at most 4 u32 of the sum so far each, as in gemm_bound; then come the
+    ceil(K / 2048) parts, and at most 8 of a cluster, with a rounding each."""
+    got, want, mags = long_product(cuda, cmb, m, n, k, 128, "f32", signed)
+    parts = -(-k // 2048) + 8
+    err = np.abs(got - want)
+    assert (err <= (4 * 64 + parts + 1) * ref.U32 * mags).all()
+    if not signed:
+        # the sums so far of terms that are positive and alike average half the
+        # last one, in an accumulator and over the parts
+        room = (4 * 64 + parts + 1) / 2 * ref.U32 * np.linalg.norm(want)
+        assert np.linalg.norm(err) <= room, np.linalg.norm(err) / np.linalg.norm(want) / ref.U32
