@@ -24,9 +24,9 @@
 //
 // The tensor core adds to its fp32 accumulator by truncation, so a sum's error
 // grows with K: 5.5e-7 of C (2-norm) at K = 2048, 2.7e-6 at 8192, against 3.6e-7
-// for the same sums rounded to nearest.  A bf16 C does not show it; for an fp32 C
-// an accumulator takes at most 16 K blocks (kSumBlocks) and the parts are added
-// in registers, rounded to nearest.
+// for the same sums rounded to nearest.  For an fp32 C an accumulator takes at most
+// 16 K blocks (kSumBlocks), for a bf16 C, which shows less, 256 (kSumBlocksBf16), and
+// the parts are added in registers, rounded to nearest.
 //
 // Two kernels: k_gemm_pair for many tokens (tensor core and L2 delivery
 // bound), k_gemm_split for few (bound by reading the weights once).
@@ -74,8 +74,13 @@ constexpr int kScaleCol = 480;          // TMEM columns of the scales: 2 x 4 and
 constexpr size_t kSmemMost = 227 * 1024 - 1024;  // less what is static
 constexpr size_t kSmemHalf = 112 * 1024;         // two CTAs a SM
 constexpr int kSplitThreads = 256;
-// K blocks of an accumulator where C is fp32: as many as share a fetch of scales
+// K blocks of an accumulator where C is fp32: as many as share a fetch of scales.
 constexpr int kSumBlocks = 16;
+// The same for a bf16 C.  32 of K are off by at most 4 u32 of the sum so far (2 for
+// the addition and 2 for the products' alignment, both downwards; of positive terms
+// that averages half the last), so 32768 of K by 2^-13 of C, 1/32 of the largest
+// rounding to bf16.
+constexpr int kSumBlocksBf16 = 256;
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d) {
@@ -233,7 +238,7 @@ __device__ __forceinline__ void store_c(const Args &g, int t, int w, float v) {
 // 4096 x 8192 10.7 us (34 MB, 5.2 us).
 // kParts: where TMEM does not hold an accumulator for each kSumBlocks K blocks,
 // two of them take turns, one for each 16 K blocks whose scales come together, and
-// warps 4-7 keep the sum, as in k_gemm_pair<true>.  The sum's 128 registers a thread
+// warps 4-7 keep the sum, as in k_gemm_pair.  The sum's 128 registers a thread
 // leave room for one CTA a SM, as so many accumulators do.
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-7 accumulators
 template <bool kParts>
@@ -515,10 +520,11 @@ __device__ __forceinline__ void tile_at(int t, int tiles_w, int tiles_t, int &tw
 // back to back, when the SM clock falls from 1.4 to 1.1-1.3 GHz.  L2 hands
 // the SMs 4.9 GB meanwhile.  Wider tiles (256 x 448 in two parts of TMEM, 256 x
 // 480) read less but store with no MMAs beside: 395 and 400 us.
-// kSums (fp32 C, n <= 224): each kSumBlocks K blocks of a tile go to the next of
-// the two accumulators, and the warps that read them keep the sum.
+// kPart > 0: each kPart K blocks of a tile go to the next of the accumulators, and the
+// warps that read them keep the sum.  A bf16 C then has one at n = 256, which 256 K
+// blocks (50 us) wait for no more than 1 us; an fp32 C stays at n <= 224.
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-11 accumulators
-template <bool kSums>
+template <int kPart>
 __global__ void __launch_bounds__(kPairThreads, 1)
     k_gemm_pair(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_t,
                 const Args g) {
@@ -613,7 +619,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         int a = 0, from = 0;  // the accumulator and its first K block
         uint32_t d = 0;
         for (int b = 0; 4 * b < g.groups && ok; ++b, ++i) {
-          if (b == 0 || (kSums && 4 * b % kSumBlocks == 0)) {
+          if (b == 0 || (kPart && 4 * b % (kPart + !kPart) == 0)) {
             a = j % bufs, from = 4 * b, d = tmem + a * n;
             ok = wait.of_pair(&tempty[a], (static_cast<uint32_t>(j / bufs) & 1) ^ 1);
             if (!ok) break;
@@ -658,7 +664,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (dev::elect_one()) {
             tc::commit<2>(dev::smem_addr(&bdone[slot]));
             if (last) tc::commit_pair(dev::smem_addr(&sfree[buf]));
-            if (kend == g.groups || (kSums && kend % kSumBlocks == 0))
+            if (kend == g.groups || (kPart && kend % (kPart + !kPart) == 0))
               tc::commit_pair(dev::smem_addr(&tfull[a]));
           }
           __syncwarp();
@@ -707,7 +713,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int tw, tt;
       tile_at(t, tiles_w, tiles_t, tw, tt);
       const int w = tw * 256 + rank * 128 + q * 32 + lane;
-      if constexpr (!kSums) {
+      if constexpr (kPart == 0) {
         const int a = j % bufs;
         ok = wait(&tfull[a], static_cast<uint32_t>(j / bufs) & 1);
         if (!ok) break;
@@ -722,16 +728,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         ++j;
       } else {
-        // this warp's chunks of 16 columns are h, h + 2, ...: at most 7
-        uint32_t sum[7][16];
-        for (int from = 0; from < g.groups && ok; from += kSumBlocks, ++j) {
+        // this warp's chunks of 16 columns: h, h + 2, ...
+        constexpr int kChunks = kPart == kSumBlocks ? 7 : 8;
+        uint32_t sum[kChunks][16];
+        for (int from = 0; from < g.groups && ok; from += kPart, ++j) {
           const int a = j % bufs;
           ok = wait(&tfull[a], static_cast<uint32_t>(j / bufs) & 1);
           if (!ok) break;
           tc::fence_after_sync();
           const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + a * n + 16 * h;
 #pragma unroll
-          for (int c = 0; c < 7; ++c) {
+          for (int c = 0; c < kChunks; ++c) {
             if (h + 2 * c >= chunks) continue;
             if (from == 0) {
               tc::ld_32x32b_x16(at + 32 * c, sum[c]);
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < 7; ++c)
+        for (int c = 0; c < kChunks; ++c)
           if (h + 2 * c < chunks) store_columns<16>(g, tt * n + 16 * (h + 2 * c), w, sum[c]);
       }
     }
@@ -912,20 +919,23 @@ int launch(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
            cudaStream_t stream) {
   Cut cut = choose_cut(g, lda % 128 != 0 || ldb % 128 != 0);
   g.n = cut.n;
+  const int most = g.bf16 ? kSumBlocksBf16 : kSumBlocks;  // K blocks of an accumulator
   if (cut.split == 0) {
     const long long tiles = tiles_of(g, 256, g.n);
     if (tiles > 0x3fffffffLL) return fail(CMB_ERR_INVALID_ARG, "gemm: too many tiles");
     const int pairs = current_sm_count() / 2;
     const long long ctas = 2 * (tiles < pairs ? tiles : pairs);
-    auto kernel = !g.bf16 && g.groups > kSumBlocks ? k_gemm_pair<true> : k_gemm_pair<false>;
+    auto kernel = g.groups <= most ? k_gemm_pair<0>
+                  : g.bf16         ? k_gemm_pair<kSumBlocksBf16>
+                                   : k_gemm_pair<kSumBlocks>;
     return launch_kernel(kernel, A, lda, B, ldb, g, g.n / 2, ctas, 2, kPairThreads, kScaleSlot,
                          kSmemMost, stream);
   }
   g.split = cut.split;
-  // one accumulator for each kSumBlocks of a CTA's K blocks where C is fp32: in
-  // half of TMEM or (one CTA a SM) all of it, or two that take turns
+  // an accumulator for each `most` of a CTA's K blocks: in half of TMEM or (one CTA a
+  // SM) all of it, or two that take turns
   const int blocks = (g.groups + g.split - 1) / g.split;
-  g.sums = g.bf16 ? 1 : (blocks + kSumBlocks - 1) / kSumBlocks;
+  g.sums = (blocks + most - 1) / most;
   if (g.sums > (256 - 16) / g.n) cut.two = false;
   const bool parts = g.sums > (512 - 16) / g.n;
   if (parts) g.sums = 2;

@@ -315,7 +315,9 @@ int cmb_quantize_e4m3_block128(const void *src, int src_type, int rows, int cols
  * time where their rows start on 16 bytes (a pitch that is a multiple of 16),
  * so a row's last piece may read behind its last scale, but not use it, up to
  * the next multiple of 16.  An fp32 C adds accumulators of at most 2048 of K
- * rounded to nearest, since the tensor core's own additions truncate.  The die map is not used: the result
+ * rounded to nearest, since the tensor core's own additions truncate; a bf16 C adds
+ * accumulators of at most 32768, off by 2^-13 of C at most where the terms of a sum are
+ * alike (its own rounding: 2^-8).  The die map is not used: the result
  * does not depend on it.  *status (device, may be NULL) is not cleared: it
  * keeps the first CMB_ERR_TIMEOUT of any call since the caller zeroed it, so a
  * program reads it once for many products. */

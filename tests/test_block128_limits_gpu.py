@@ -119,7 +119,8 @@ def long_values(q, s, rows, k, block):
 
 
 def long_product(cuda, cmb, m, n, k, block_b, out, signed):
-    """The product, and its rows and columns that are compared: ends and a few."""
+    """Of the product the rows and columns that are compared (the ends and a few), the
+    same in 64 bits, the same of magnitudes; and all of it as it is."""
     a, b = long_operand(cuda, m, k, 1, 1, signed), long_operand(cuda, n, k, block_b, 2, signed)
     c = cuda.full((m, n), float("nan"), dtype=cuda.bfloat16 if out == "bf16" else cuda.float32,
                   device="cuda")
@@ -134,7 +135,7 @@ def long_product(cuda, cmb, m, n, k, block_b, out, signed):
     got = f64(c[cuda.from_numpy(rows).cuda()][:, cuda.from_numpy(cols).cuda()])
     x = long_values(*a, rows, k, 1)
     y = long_values(*b, cols, k, block_b)
-    return got, x @ y.T, np.abs(x) @ np.abs(y).T
+    return got, x @ y.T, np.abs(x) @ np.abs(y).T, c
 
 
 # few tokens and many, one CTA a tile and up to eight, whole and odd sizes
@@ -149,7 +150,7 @@ def test_gemm_fp32_sums_of_any_length(cuda, cmb, m, n, k, signed):
     """An fp32 C adds accumulators of 2048 of K.  An accumulator's 64 MMAs are off
     by at most 4 u32 of the sum so far each, as in gemm_bound; then come the
     ceil(K / 2048) parts, and at most 8 of a cluster, with a rounding each."""
-    got, want, mags = long_product(cuda, cmb, m, n, k, 128, "f32", signed)
+    got, want, mags, _ = long_product(cuda, cmb, m, n, k, 128, "f32", signed)
     parts = -(-k // 2048) + 8
     err = np.abs(got - want)
     assert (err <= (4 * 64 + parts + 1) * ref.U32 * mags).all()
@@ -158,3 +159,35 @@ def test_gemm_fp32_sums_of_any_length(cuda, cmb, m, n, k, signed):
         # last one, in an accumulator and over the parts
         room = (4 * 64 + parts + 1) / 2 * ref.U32 * np.linalg.norm(want)
         assert np.linalg.norm(err) <= room, np.linalg.norm(err) / np.linalg.norm(want) / ref.U32
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 2048, 131072), (128, 9472, 100003), (3000, 3000, 40000),
+                                   (16, 256, 2 ** 22), (5, 8192, 2 ** 18), (300, 600, 32768)])
+@pytest.mark.parametrize("signed", [False, True])
+def test_gemm_bf16_sums_of_any_length(cuda, cmb, m, n, k, signed):
+    """A bf16 C is off by its own rounding and little else: it adds accumulators of at
+    most 32768 of K, each off by at most 4 u32 of the sum so far for each 32, and at
+    most 8 of a cluster."""
+    got, want, mags, _ = long_product(cuda, cmb, m, n, k, 128, "bf16", signed)
+    steps = 4 * 1024 + -(-k // 32768) + 8
+    room = steps * ref.U32 * mags + ref.U16 * np.abs(want) * (1 + 1e-3)
+    assert (np.abs(got - want) <= room).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1024, 1024, 2 ** 19), (2000, 2100, 300001), (128, 4800, 2 ** 19),
+                                   (16, 4096, 2 ** 20), (48, 8000, 2 ** 19 - 77)])
+def test_gemm_bf16_sums_do_not_drift(cuda, cmb, m, n, k):
+    """Positive terms and K past 8 x 32768, so that every CTA of a cluster has more
+    than one accumulator of a bf16 C.  Against the fp32 C of the same operands the
+    mean difference is that of the sums, (4096 + parts) / 2 and (256 + parts) / 2 u32
+    of C by the same count as in the fp32 test, and what is left of the roundings to
+    bf16: each is uniform within half a step, at most 2^-8 of C, a third of its
+    square on average, and six deviations of the mean of all of them are allowed
+    for."""
+    sums = {}
+    for out in ("bf16", "f32"):
+        sums[out] = long_product(cuda, cmb, m, n, k, 128, out, False)[3].double()
+    drift = float((sums["bf16"] / sums["f32"] - 1).mean())
+    room = (4 * 1024 + 4 * 64 + -(-k // 32768) + -(-k // 2048) + 16) / 2 * ref.U32
+    room += 6 * ref.U16 / np.sqrt(3 * m * n)
+    assert abs(drift) <= room, (drift / ref.U32, room / ref.U32)
