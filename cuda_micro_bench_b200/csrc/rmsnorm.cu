@@ -50,6 +50,24 @@ __device__ __forceinline__ float row_sum(float v, float *part) {
   return v;
 }
 
+constexpr int kNever = 0x7FFFFFFF;
+
+// A wait for turn `turn` that was not over at once.  Where it runs out, or one of the
+// CTA has, the thread goes on with what the stage holds, and the CTA gives up its
+// rows from that turn on once it is through them (Ring::failed).
+static __device__ __noinline__ void wait_long(uint32_t bar, uint32_t parity, int turn,
+                                              int *failed_at) {
+  const uint64_t deadline = dev::globaltimer() + dev::kWaitLimitNs;
+#pragma unroll 1
+  while (!dev::mbar_try_wait(bar, parity)) {
+    if (*const_cast<volatile int *>(failed_at) != kNever) return;
+    if (dev::globaltimer() > deadline) {
+      atomicMin(failed_at, turn);
+      return;
+    }
+  }
+}
+
 // Rows of up to three matrices on their way through shared memory.  A CTA's
 // turn i is over rows (blockIdx.x + i * gridDim.x) * blockDim.y and on, in stage
 // i % kStages.
@@ -60,10 +78,19 @@ struct Ring {
   uint32_t bytes;  // of a row of one of them
   uint8_t *mem;
   uint64_t *full;
+  int *failed_at;  // the first turn whose wait has run out, and the first not loaded for it
 
+  __device__ __forceinline__ long long first_row(int i) const {
+    return (blockIdx.x + static_cast<long long>(i) * gridDim.x) * blockDim.y;
+  }
+  // By one thread, whose own waits tell it that the turn's place is free.
   __device__ __forceinline__ void load(int i, int rows) const {
-    const long long first = (blockIdx.x + static_cast<long long>(i) * gridDim.x) * blockDim.y;
+    const long long first = first_row(i);
     if (first >= rows) return;
+    if (*const_cast<volatile int *>(failed_at) != kNever) {
+      failed_at[1] = min(failed_at[1], i);
+      return;
+    }
     const int high = static_cast<int>(min(static_cast<long long>(blockDim.y), rows - first));
     const int s = i % kStages;
     const uint32_t bar = dev::smem_addr(full + s);
@@ -76,15 +103,32 @@ struct Ring {
     if (threadIdx.x == 0 && threadIdx.y == 0) {
       for (int s = 0; s < kStages; ++s) dev::mbar_init(dev::smem_addr(full + s), 1);
       dev::fence_mbar_init();
+      failed_at[0] = failed_at[1] = kNever;
     }
     __syncthreads();
     if (threadIdx.x == 0 && threadIdx.y == 0)
       for (int s = 0; s < kStages; ++s) load(s, rows);
   }
-  // Waits for turn i; a bulk copy of this GPU's own memory ends, or the launch
-  // has failed as a whole.
   __device__ __forceinline__ void wait(int i) const {
-    dev::mbar_wait_bounded(dev::smem_addr(full + i % kStages), (i / kStages) & 1);
+    const uint32_t bar = dev::smem_addr(full + i % kStages), parity = (i / kStages) & 1;
+    if (!dev::mbar_try_wait(bar, parity)) wait_long(bar, parity, i, failed_at);
+  }
+  // All threads, when they are through their rows: whether a wait has run out.  The
+  // copies that are still on their way then land (or their waits run out too), and
+  // `row` is the first that the CTA gives up.
+  __device__ __forceinline__ bool failed(int rows, int &row) const {
+    __syncthreads();
+    const int turn = failed_at[0];
+    if (turn == kNever) return false;
+    row = static_cast<int>(first_row(turn));
+    if (threadIdx.x == 0 && threadIdx.y == 0) {
+      int end = 0;
+      while (end < failed_at[1] && first_row(end) < rows) ++end;
+      for (int i = max(0, end - kStages); i < end; ++i)
+        dev::mbar_wait_bounded(dev::smem_addr(full + i % kStages), (i / kStages) & 1, 100000000ull);
+    }
+    __syncthreads();
+    return true;
   }
   __device__ __forceinline__ uint8_t *at(int s, int y, int k) const {
     return mem + static_cast<size_t>((s * static_cast<int>(blockDim.y) + y) * n + k) * bytes;
@@ -94,6 +138,20 @@ struct Ring {
     return reinterpret_cast<const T *>(at(i % kStages, threadIdx.y, k));
   }
 };
+
+// What the CTA's rows from `first` on read where a wait has run out: `word` over all
+// of them, `bytes` (a multiple of 8, as the rows' starts are) each.
+static __device__ __noinline__ void spoil_rows(void *p, size_t pitch, uint32_t bytes, uint32_t word,
+                                               int first, int rows) {
+  if (p == nullptr) return;
+  for (; first < rows; first += gridDim.x * blockDim.y) {
+    const int row = first + threadIdx.y;
+    if (row >= rows) return;
+    uint2 *to = reinterpret_cast<uint2 *>(static_cast<uint8_t *>(p) + row * pitch);
+    for (uint32_t i = threadIdx.x; i < bytes / 8; i += blockDim.x) to[i] = make_uint2(word, word);
+  }
+}
+constexpr uint32_t kNanWord = 0x7FFF7FFFu;  // NaN as two bf16 and as a fp32
 
 // 8 columns of a row, from the ring or from where the row lies.
 template <typename T, int kWay>
@@ -199,6 +257,7 @@ template <typename T, typename W, int NV, int kWay>
 __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
   __shared__ float part[2][32];
   __shared__ __align__(8) uint64_t full[kStages];
+  __shared__ int failed_at[2];
   extern __shared__ __align__(16) uint8_t rows_mem[];
   dev::grid_dep_wait();
   dev::grid_dep_launch();
@@ -209,7 +268,8 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
             a.residual != nullptr ? 2 : 1,
             static_cast<uint32_t>(a.cols * sizeof(T)),
             rows_mem,
-            full};
+            full,
+            failed_at};
     ring.start(a.rows);
   }
   Bounds in_x{}, in_r{};
@@ -265,6 +325,21 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm(const NormArgs a) {
       if (a.q != nullptr) store_quantized<kWay>(a, row, col, n, y);
     }
   }
+  if constexpr (kWay == kRing) {
+    int row;
+    if (ring.failed(a.rows, row)) {
+      const uint32_t bytes = a.cols * sizeof(T);
+      spoil_rows(a.h, a.ld_h * sizeof(T), bytes, kNanWord, row, a.rows);
+      spoil_rows(a.y, a.ld_y * sizeof(T), bytes, kNanWord, row, a.rows);
+      spoil_rows(a.q, a.ld_q, a.cols, 0x7F7F7F7Fu, row, a.rows);
+      for (row += threadIdx.y; row < a.rows; row += gridDim.x * blockDim.y) {
+        if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = __uint_as_float(kNanWord);
+        if (a.q != nullptr)
+          for (int g = threadIdx.x; g < b128::groups_of(a.cols); g += blockDim.x)
+            a.scale[static_cast<size_t>(row) * a.ld_scale + g] = 255;
+      }
+    }
+  }
 }
 
 struct NormBackArgs {
@@ -284,6 +359,7 @@ template <typename T, typename W, int NV, int kWay>
 __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) {
   __shared__ float part[2][32];
   __shared__ __align__(8) uint64_t full[kStages];
+  __shared__ int failed_at[2];
   extern __shared__ __align__(16) uint8_t rows_mem[];
   dev::grid_dep_wait();
   dev::grid_dep_launch();
@@ -295,7 +371,8 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
             a.dh != nullptr ? 3 : 2,
             static_cast<uint32_t>(a.cols * sizeof(T)),
             rows_mem,
-            full};
+            full,
+            failed_at};
     ring.start(a.rows);
   }
   Bounds in_dy{}, in_h{}, in_dh{};
@@ -350,6 +427,16 @@ __global__ void __launch_bounds__(1024, 1) k_rmsnorm_back(const NormBackArgs a) 
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[j] = fmaf(rstd, fmaf(u[j], minus, g[j]), past[j]);
       store_chunk<T, kWay>(a.dx, a.ld_dx, row, col, n, b128::packed<T>(g));
+    }
+  }
+  if constexpr (kWay == kRing) {
+    int row;
+    if (ring.failed(a.rows, row)) {
+      spoil_rows(a.dx, a.ld_dx * sizeof(T), a.cols * sizeof(T), kNanWord, row, a.rows);
+      if (a.parts != nullptr)  // and with them all of dweight
+        spoil_rows(a.parts + static_cast<size_t>(blockIdx.x) * a.ld_parts, 0,
+                   a.ld_parts * sizeof(float), kNanWord, 0, 1);
+      return;
     }
   }
   if (a.parts == nullptr) return;

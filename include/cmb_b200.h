@@ -338,8 +338,10 @@ int cmb_gemm_e4m3_block128(const uint8_t *A, size_t lda, const uint8_t *scale_a,
  * q, scale may be NULL.  But for h, no output may overlap an input or another
  * output.  rows = 0 writes nothing.  Sums are fp32: a row whose squares overflow
  * (values past 1e18 or so) has rstd 0; with eps 0, rows under 1e-19 lose bits with
- * their squares, and one whose squares are all 0 has rstd infinite and NaN in y.
- * Rows that start on 16 bytes, with cols a multiple of 8, are fastest. */
+ * their squares, and one whose squares are all 0 has rstd infinite and no finite y.
+ * Rows that start on 16 bytes, with cols a multiple of 8, are fastest.  Should a
+ * wait for such rows run out (2 s), the rows that wait for one another hold NaN from
+ * there on in every output (q 0x7F, scale 255). */
 #define CMB_RMSNORM_MAX_COLS 32768
 int cmb_rmsnorm_e4m3_block128(const void *x, size_t ld_x, const void *residual, size_t ld_residual,
                               int type, const void *weight, int weight_type, float eps, int rows,
@@ -360,7 +362,8 @@ size_t cmb_rmsnorm_backward_workspace_bytes(int rows, int cols);
  * dweight may be NULL, and workspace with it; otherwise workspace is
  * cmb_rmsnorm_backward_workspace_bytes(rows, cols) bytes of device memory,
  * 16-byte aligned, that need no initialisation; two calls whose work overlaps
- * on the GPU need separate workspaces.  rows = 0 sets dweight to zeros. */
+ * on the GPU need separate workspaces.  rows = 0 sets dweight to zeros.  A wait
+ * that runs out leaves NaN as above in dx, and in all of dweight. */
 int cmb_rmsnorm_backward(const void *dy, size_t ld_dy, const void *h, size_t ld_h, const void *dh,
                          size_t ld_dh, int type, const void *weight, int weight_type,
                          const float *rstd, int rows, int cols, void *dx, size_t ld_dx,

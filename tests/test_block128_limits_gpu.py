@@ -3,6 +3,9 @@ without an argument of it being unusual: two host threads at once, long sums,
 rows near the ends of fp32, waits that run out."""
 
 import ctypes
+import glob
+import os
+import subprocess
 import threading
 
 import numpy as np
@@ -191,3 +194,82 @@ def test_gemm_bf16_sums_do_not_drift(cuda, cmb, m, n, k):
     room = (4 * 1024 + 4 * 64 + -(-k // 32768) + -(-k // 2048) + 16) / 2 * ref.U32
     room += 6 * ref.U16 / np.sqrt(3 * m * n)
     assert abs(drift) <= room, (drift / ref.U32, room / ref.U32)
+
+
+# --------------------------------------------------- a wait that runs out
+
+
+class Lost:
+    """The norms of tests/lost_copy.cu, called as the library's."""
+
+    def __init__(self, lib, signatures):
+        self.lib = lib
+        for name in ("cmb_rmsnorm_e4m3_block128", "cmb_rmsnorm_backward",
+                     "cmb_rmsnorm_backward_workspace_bytes"):
+            f = getattr(lib, name)
+            f.restype, f.argtypes = signatures[name]
+
+    def check(self, name, *args):
+        assert getattr(self.lib, name)(*args) == 0
+
+    def lose(self, address):
+        assert self.lib.lose_row(ctypes.c_uint64(address)) == 0
+
+
+@pytest.fixture(scope="module")
+def lost(cuda, cmb, tmp_path_factory):
+    from cuda_micro_bench_b200 import capi
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    home = os.path.join(root, "cuda_micro_bench_b200")
+    out = str(tmp_path_factory.mktemp("lost") / "liblost.so")
+    objects = [o for o in glob.glob(home + "/_obj/**/*.o", recursive=True)
+               if os.path.basename(o) != "rmsnorm.cu.o"]
+    subprocess.run(["/usr/local/cuda/bin/nvcc", "-O3", "-std=c++17", "-gencode",
+                    "arch=compute_100a,code=sm_100a", "-Xcompiler", "-fPIC", "-shared", "-Xlinker",
+                    "-Bsymbolic", "-I", home + "/csrc", "-I", root + "/include",
+                    os.path.join(root, "tests", "lost_copy.cu"), *objects, "-lpthread", "-ldl",
+                    "-o", out], check=True, timeout=600)
+    return Lost(ctypes.CDLL(out), capi.SIGNATURES)
+
+
+@pytest.mark.parametrize("rows,cols,row", [(1500, 8192, 777), (1500, 8192, 0), (1500, 1032, 1499)])
+def test_norm_whose_wait_runs_out(cuda, cmb, lost, rows, cols, row):
+    """A row's copy never comes (a wait ends after 2 s): the row and what its CTA
+    has left hold NaN in every output, all other rows are right, and the next
+    call works."""
+    rng = np.random.default_rng(rows)
+    x, r = (on_gpu(cuda, rng.normal(size=(rows, cols)), "bf16")[1] for _ in range(2))
+    w = on_gpu(cuda, np.ones((1, cols)), "bf16")[1]
+    call = lambda: run_norm(cuda, lost, x, r, w, "bf16", "bf16", 1e-5)
+    want = run_norm(cuda, cmb, x, r, w, "bf16", "bf16", 1e-5)
+    lost.lose(r.data_ptr() + 2 * cols * row)
+    got = call()
+    lost.lose(0)
+    again = call()
+    spoilt = cuda.isnan(got["rstd"])
+    assert bool(spoilt[row]) and int(spoilt[:row].sum()) <= 1  # rows are taken in order, two at a time
+    assert int(spoilt.sum()) <= 64  # of one CTA
+    for name in ("h", "y"):
+        assert cuda.isnan(got[name][spoilt]).all()
+    assert (got["q"][spoilt] == 0x7F).all() and (got["s"][spoilt] == 255).all()
+    for name in ("h", "y", "q", "s", "rstd"):
+        assert cuda.equal(got[name][~spoilt], want[name][~spoilt]), name
+        assert cuda.equal(again[name], want[name]), name
+
+
+@pytest.mark.parametrize("rows,cols,row", [(1500, 8192, 777), (1500, 8192, 0), (1500, 1032, 1499)])
+def test_gradient_whose_wait_runs_out(cuda, cmb, lost, rows, cols, row):
+    rng = np.random.default_rng(rows)
+    dy, h, dh, w, rstd = backward_inputs(cuda, rng, rows, cols, "bf16", "bf16")
+    call = lambda c: run_backward(cuda, c, dy, h, dh, w, rstd, "bf16", "bf16")
+    want = call(cmb)
+    lost.lose(h.data_ptr() + 2 * cols * row)
+    dx, grad = call(lost)
+    lost.lose(0)
+    again = call(lost)
+    spoilt = cuda.isnan(dx).any(dim=1)
+    assert bool(spoilt[row]) and int(spoilt[:row].sum()) <= 1 and int(spoilt.sum()) <= 64
+    assert cuda.isnan(dx[spoilt]).all() and cuda.isnan(grad).all()
+    assert cuda.equal(dx[~spoilt], want[0][~spoilt])
+    assert cuda.equal(again[0], want[0]) and cuda.equal(again[1], want[1])
