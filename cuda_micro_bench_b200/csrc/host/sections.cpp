@@ -19,6 +19,7 @@
 
 #include "../../../include/cmb_b200.h"
 #include "../cmb_host.h"
+#include "block128_check.h"
 #include "result_logger.h"
 
 namespace cmb {
@@ -773,8 +774,8 @@ int section_tensor_core() {
 namespace {
 
 // The calls of one e4m3 linear layer of 8192 tokens x 8192 x 8192 with a scale
-// for each block of 128 values: norm with residual, product, the norm's
-// gradient; each timed and checked on samples against fp64.
+// for each block of 128 values: quantiser, norm with residual, product, the
+// norm's gradient; each timed and every output checked on samples against fp64.
 int fp8_linear_layer() {
   const int n = 8192, groups = n / 128;
   const size_t nn = (size_t)n * n;
@@ -851,14 +852,35 @@ int fp8_linear_layer() {
                std::ldexp(1.0, hws[(size_t)(row / 128) * groups + k / 128] - 127);
       },
       hc, n, n, n, 8);
-  if (err > 1e-2)
-    return fail(CMB_ERR_MISMATCH, "block-scaled GEMM: sampled rel err %.3g > 1e-2", err);
+  // accumulators of 2048 of K are off by ~5e-7 of C; 1e-5 of the tile's largest
+  // leaves no room for longer ones or for a lost K block
+  if (!(err <= 1e-5))
+    return fail(CMB_ERR_MISMATCH, "block-scaled GEMM: sampled rel err %.3g > 1e-5", err);
+
+  // Eight blocks of the weights, exactly.
+  std::vector<uint16_t> block(128 * 128);
+  uint64_t lcg = 12345;
+  for (int i = 0; i < 8; ++i) {
+    lcg = lcg * 6364136223846793005ull + 1442695040888963407ull;
+    const int br = i == 0 ? 0 : i == 1 ? groups - 1 : static_cast<int>((lcg >> 33) % groups);
+    const int bc = i == 0 ? 0 : i == 1 ? groups - 1 : static_cast<int>((lcg >> 13) % groups);
+    const size_t at = (size_t)br * 128 * n + (size_t)bc * 128;
+    CMB_CUDA_TRY(cudaMemcpy2D(block.data(), 256, w.as<uint16_t>() + at, (size_t)n * 2, 256, 128,
+                              cudaMemcpyDeviceToHost));
+    if (!check::block_holds([&](int row, int k) { return bf16_bits_to_float(block[row * 128 + k]); },
+                            [&](int row, int k) { return hwq[at + (size_t)row * n + k]; },
+                            hws[(size_t)br * groups + bc], 128, 128))
+      return fail(CMB_ERR_MISMATCH, "quantise: block %d, %d of the weights is off", br, bc);
+  }
 
   // Four rows of the norm and of its gradient against fp64: e4m3 is off by at
   // most 2^-4 of a value or half a subnormal step, bf16 by 2^-8, and the fp32
   // statistics by far less.
   std::vector<uint16_t> row_x(n), row_r(n), row_h(n), row_d(n), g(n);
   CMB_CUDA_TRY(cudaMemcpy(g.data(), gain.p, n * 2, cudaMemcpyDeviceToHost));
+  std::vector<float> row_rstd(n), hdgain(n);
+  CMB_CUDA_TRY(cudaMemcpy(row_rstd.data(), rstd.p, n * 4, cudaMemcpyDeviceToHost));
+  CMB_CUDA_TRY(cudaMemcpy(hdgain.data(), dgain.p, n * 4, cudaMemcpyDeviceToHost));
   for (int i = 0; i < 4; ++i) {
     const size_t at = (size_t)(i * 2730) * n;
     auto fetch = [&](std::vector<uint16_t> &to, const DevBuf &from) {
@@ -879,6 +901,16 @@ int fp8_linear_layer() {
       along += (double)bf16_bits_to_float(row_r[k]) * bf16_bits_to_float(g[k]) * v;
     }
     const double rs = 1.0 / std::sqrt(sq / n + eps);
+    if (!(std::fabs(row_rstd[at / n] - rs) <= 1e-5 * rs))
+      return fail(CMB_ERR_MISMATCH, "rmsnorm: rstd = %g for %g", (double)row_rstd[at / n], rs);
+    for (int g0 = 0; g0 < groups; ++g0) {
+      double top = 0;
+      for (int k = 128 * g0; k < 128 * g0 + 128; ++k)
+        top = std::max(top, std::fabs(bf16_bits_to_float(row_h[k]) * rs * bf16_bits_to_float(g[k])));
+      const int s = hxs[at / n * groups + g0];
+      if (s < check::scale_byte(top * (1 - 1e-5)) || s > check::scale_byte(top * (1 + 1e-5)))
+        return fail(CMB_ERR_MISMATCH, "rmsnorm: scale byte %d for a block up to %g", s, top);
+    }
     for (int k = 0; k < n; ++k) {
       const double v = bf16_bits_to_float(row_h[k]), gk = bf16_bits_to_float(g[k]);
       const double y = v * rs * gk;
@@ -894,6 +926,26 @@ int fp8_linear_layer() {
         return fail(CMB_ERR_MISMATCH, "rmsnorm backward: %g for dx = %g",
                     (double)bf16_bits_to_float(row_d[k]), d);
     }
+  }
+  // Four stretches of 16 columns of the weight gradient.  A term meets a rounding
+  // for each row of its CTA (at least 128 CTAs share them), one for each 32nd CTA
+  // and the tree's.
+  std::vector<uint16_t> col_d((size_t)n * 16), col_h((size_t)n * 16);
+  for (int i = 0; i < 4; ++i) {
+    const int c0 = i == 3 ? n - 16 : i * 2720;
+    CMB_CUDA_TRY(cudaMemcpy2D(col_d.data(), 32, r.as<uint16_t>() + c0, (size_t)n * 2, 32, n,
+                              cudaMemcpyDeviceToHost));
+    CMB_CUDA_TRY(cudaMemcpy2D(col_h.data(), 32, h.as<uint16_t>() + c0, (size_t)n * 2, 32, n,
+                              cudaMemcpyDeviceToHost));
+    for (int c = 0; c < 16; ++c)
+      if (!check::sum_holds(hdgain[c0 + c],
+                            [&](int row) {
+                              return (double)bf16_bits_to_float(col_d[(size_t)row * 16 + c]) *
+                                     bf16_bits_to_float(col_h[(size_t)row * 16 + c]) * row_rstd[row];
+                            },
+                            n, n / 128 + 64))
+        return fail(CMB_ERR_MISMATCH, "rmsnorm backward: dweight[%d] = %g", c0 + c,
+                    (double)hdgain[c0 + c]);
   }
   const double tf = 2.0 * n * nn / (ms_g * 1e-3) / 1e12;
   const double gq = 3.0 * nn / (ms_q * 1e-3) / 1e9, gn = 7.0 * nn / (ms_n * 1e-3) / 1e9,

@@ -169,8 +169,8 @@ def check(doc, full=True, keys=None):
         bound("fp8_block128", key, 0, hbm, "HBM3e bandwidth")
     flag("fp8_block128", "verified")
     err = val("fp8_block128", "gemm_8192_max_rel_err")
-    if err is not None and err > 1e-2:
-        fail(f"fp8_block128.gemm_8192_max_rel_err = {err} above 1e-2")
+    if err is not None and err > 1e-5:
+        fail(f"fp8_block128.gemm_8192_max_rel_err = {err} above 1e-5")
     dies = [val("tensor_core_tcgen05", f"sms_on_die{d}") for d in (0, 1)]
     if all(x is not None for x in dies) and (min(dies) <= 0 or sum(dies) != B200["sm_count"]):
         fail(f"tensor_core_tcgen05.sms_on_die0/1 = {dies[0]} / {dies[1]}: not a split of "
