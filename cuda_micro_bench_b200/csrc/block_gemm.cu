@@ -236,10 +236,13 @@ __device__ __forceinline__ void store_c(const Args &g, int t, int w, float v) {
 // Bound by reading the weights: 1 x 8192 x 8192 takes 13.8 us (67 MB, 10.2 us at
 // the copy rate; 2-3 us of it are the launch and the pipe's start and end), 48 x
 // 4096 x 8192 10.7 us (34 MB, 5.2 us).
-// kParts: where TMEM does not hold an accumulator for each kSumBlocks K blocks,
-// two of them take turns, one for each 16 K blocks whose scales come together, and
-// warps 4-7 keep the sum, as in k_gemm_pair.  The sum's 128 registers a thread
-// leave room for one CTA a SM, as so many accumulators do.
+// kParts: where TMEM does not hold an accumulator for each kSumBlocks (bf16 C:
+// kSumBlocksBf16) K blocks, two of them take turns, one for each 16 K blocks whose
+// scales come together, and warps 4-7 keep the sum, as in k_gemm_pair.  The sum's 128
+// registers a thread leave room for one CTA a SM, as so many accumulators do.  The
+// turns change with the batches of scales, outside the loop that issues MMAs: inside
+// it they cost 7-17 % (128 x 18944 x 16384 91 us), here within 1 % of accumulators
+// that grow with K (80).
 //   warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 4-7 accumulators
 template <bool kParts>
 __global__ void __launch_bounds__(kSplitThreads, kParts ? 1 : 2)
@@ -536,6 +539,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag;
 
+  constexpr int kEach = kPart > 0 ? kPart : 1 << 30;     // K blocks of an accumulator
   const int n = g.n, bufs = 2 * n <= kScaleCol ? 2 : 1;  // accumulators
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int rank = uniform(tc::cluster_ctarank());
@@ -619,7 +623,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         int a = 0, from = 0;  // the accumulator and its first K block
         uint32_t d = 0;
         for (int b = 0; 4 * b < g.groups && ok; ++b, ++i) {
-          if (b == 0 || (kPart && 4 * b % (kPart + !kPart) == 0)) {
+          if (4 * b % kEach == 0) {
             a = j % bufs, from = 4 * b, d = tmem + a * n;
             ok = wait.of_pair(&tempty[a], (static_cast<uint32_t>(j / bufs) & 1) ^ 1);
             if (!ok) break;
@@ -664,7 +668,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (dev::elect_one()) {
             tc::commit<2>(dev::smem_addr(&bdone[slot]));
             if (last) tc::commit_pair(dev::smem_addr(&sfree[buf]));
-            if (kend == g.groups || (kPart && kend % (kPart + !kPart) == 0))
+            if (kend == g.groups || kend % kEach == 0)
               tc::commit_pair(dev::smem_addr(&tfull[a]));
           }
           __syncwarp();
@@ -941,8 +945,9 @@ int launch(const uint8_t *A, size_t lda, const uint8_t *B, size_t ldb, Args g,
   if (parts) g.sums = 2;
   g.tmem_cols = 32;
   while (g.tmem_cols < g.sums * g.n + 16) g.tmem_cols *= 2;
-  return launch_kernel(parts ? k_gemm_split<true> : k_gemm_split<false>, A, lda, B, ldb, g, g.n, tiles_of(g, 128, g.n) * g.split,
-                       g.split, kSplitThreads, kSplitSlot, cut.two ? kSmemHalf : kSmemMost, stream);
+  return launch_kernel(parts ? k_gemm_split<true> : k_gemm_split<false>, A, lda, B, ldb, g, g.n,
+                       tiles_of(g, 128, g.n) * g.split, g.split, kSplitThreads, kSplitSlot,
+                       cut.two ? kSmemHalf : kSmemMost, stream);
 }
 
 }  // namespace
