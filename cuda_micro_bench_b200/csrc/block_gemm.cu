@@ -895,7 +895,9 @@ Cut choose_cut(const Args &g, bool skewed) {
   const int fewest = (g.t_rows + 127) / 128;
   int last = 0;
   for (int parts = fewest; parts < fewest + 8; ++parts) {
-    const int n = ((g.t_rows + parts - 1) / parts + 15) / 16 * 16;
+    // in 64 bits: parts is a 128th of up to 2^31
+    const int n = static_cast<int>((static_cast<long long>(g.t_rows) + parts - 1) / parts + 15) /
+                  16 * 16;
     if (n == last || (parts > 1 && n < 48)) continue;
     last = n;
     const long long tiles = tiles_of(g, 128, n);

@@ -273,3 +273,98 @@ def test_gradient_whose_wait_runs_out(cuda, cmb, lost, rows, cols, row):
     assert cuda.isnan(dx[spoilt]).all() and cuda.isnan(grad).all()
     assert cuda.equal(dx[~spoilt], want[0][~spoilt])
     assert cuda.equal(again[0], want[0]) and cuda.equal(again[1], want[1])
+
+
+# ------------------------------------------------------- the largest extents
+
+MOST = 2 ** 31 - 2 ** 16  # rows or columns that a call takes
+
+
+@pytest.fixture
+def space(cuda):
+    cuda.cuda.empty_cache()
+    if cuda.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free device memory")
+    yield
+    cuda.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("side", ["m", "n"])
+@pytest.mark.parametrize("k", [1, 16])
+def test_gemm_of_the_largest_extent(cuda, cmb, space, side, k):
+    """As many rows of one operand as a call takes, one of the other: 2 in the first,
+    the last and one between, 1 elsewhere, under scales of 1."""
+    long = cuda.full((MOST, 16), 0x38, dtype=cuda.uint8, device="cuda")  # 1.0
+    for row in (0, 2 ** 30 + 7, MOST - 1):
+        long[row] = 0x40  # 2.0
+    scales = cuda.full((MOST,), 127, dtype=cuda.uint8, device="cuda")
+    one, s1 = long[1:2].clone(), scales[:1].clone()
+    c = cuda.full((MOST,), 7.0, dtype=cuda.bfloat16, device="cuda")
+    status = cuda.zeros(1, dtype=cuda.int32, device="cuda")
+    m, n = (MOST, 1) if side == "m" else (1, MOST)
+    a, sa, b, sb = (long, scales, one, s1) if side == "m" else (one, s1, long, scales)
+    cmb.check("cmb_gemm_e4m3_block128", addr(a), 16, addr(sa), 1, addr(b), 16, addr(sb), 1, 1,
+              addr(c), n, BF16, m, n, k, addr(status), stream_handle(cuda))
+    assert int(status.item()) == 0
+    for row in (0, 2 ** 30 + 7, MOST - 1):
+        assert float(c[row]) == 2.0 * k
+        c[row] = 1.0 * k
+    assert float(c.min()) == float(c.max()) == k
+
+
+def test_norm_and_gradient_of_the_largest_extent(cuda, cmb, space):
+    """Rows of one value: y = sign(x) but for eps, whose share is exact here, and a
+    gradient that nothing but dh reaches."""
+    x = cuda.full((MOST,), 3.0, dtype=cuda.bfloat16, device="cuda")
+    x[0] = x[2 ** 30 + 7] = x[-1] = -3.0
+    w = cuda.ones(1, dtype=cuda.bfloat16, device="cuda")
+    y = cuda.full((MOST,), 7.0, dtype=cuda.bfloat16, device="cuda")
+    cmb.check("cmb_rmsnorm_e4m3_block128", addr(x), 1, None, 0, BF16, addr(w), BF16,
+              ctypes.c_float(0.0), MOST, 1, None, 0, addr(y), 1, None, 0, None, 0, None,
+              stream_handle(cuda))
+    for row in (0, 2 ** 30 + 7, MOST - 1):
+        assert float(y[row]) == -1.0
+        y[row] = 1.0
+    assert float(y.min()) == float(y.max()) == 1.0
+    # rstd of 1/2 and h of 2: dx = (dy - 2 (1/4) (2 dy)) / 2 = 0, and with dh = dy it is dy
+    x.fill_(2.0)
+    y[0] = y[2 ** 30 + 7] = y[-1] = 5.0
+    rstd = cuda.full((MOST,), 0.5, device="cuda")
+    dx = cuda.full((MOST,), 7.0, dtype=cuda.bfloat16, device="cuda")
+    cmb.check("cmb_rmsnorm_backward", addr(y), 1, addr(x), 1, addr(y), 1, BF16, addr(w), BF16,
+              addr(rstd), MOST, 1, addr(dx), 1, None, None, 0, stream_handle(cuda))
+    assert cuda.equal(dx, y)
+
+
+@pytest.mark.parametrize("rows,cols,block", [(MOST, 1, 1), (1, MOST, 1), (MOST, 1, 128)])
+def test_quantize_of_the_largest_extent(cuda, cmb, space, rows, cols, block):
+    x = cuda.full((MOST,), 3.0, dtype=cuda.bfloat16, device="cuda")
+    x[-1] = 6.0
+    q = cuda.full((MOST,), FILL, dtype=cuda.uint8, device="cuda")
+    high, wide = -(-rows // block), -(-cols // 128)
+    s = cuda.full((high, wide), FILL, dtype=cuda.uint8, device="cuda")
+    cmb.check("cmb_quantize_e4m3_block128", addr(x), BF16, rows, cols, cols, block, addr(q), cols,
+              addr(s), wide, None, 0, None, 0, stream_handle(cuda))
+    wq, ws = ref.quantize(np.array([[3.0]]), 1)
+    lq, ls = ref.quantize(np.array([[6.0]]), 1)  # the last block: 6 is its largest
+    assert int(s.view(-1)[-1]) == ls[0, 0] and int(q[-1]) == lq[0, 0]
+    if high * wide > 1:
+        rest = s.view(-1)[:-1]
+        assert int(rest.min()) == int(rest.max()) == ws[0, 0]
+    head = q[:MOST - 128]
+    assert int(head.min()) == int(head.max()) == wq[0, 0]
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n", [(1, 5), (33, 3)])
+def test_gemm_of_the_longest_k(cuda, cmb, space, m, n, out):
+    """K = 2^28 ones: every sum on the way is a whole number under 2^24 or a multiple
+    of 2048 up to 2^28, so C is 2^28 exactly."""
+    k = 2 ** 28
+    a, b = (cuda.full((rows, k), 0x38, dtype=cuda.uint8, device="cuda") for rows in (m, n))
+    sa, sb = (cuda.full((rows, k // 128), 127, dtype=cuda.uint8, device="cuda") for rows in (m, n))
+    c = cuda.full((m, n), 7.0, dtype=cuda.bfloat16 if out == "bf16" else cuda.float32, device="cuda")
+    status = cuda.zeros(1, dtype=cuda.int32, device="cuda")
+    cmb.check("cmb_gemm_e4m3_block128", addr(a), k, addr(sa), k // 128, addr(b), k, addr(sb),
+              k // 128, 1, addr(c), n, CODE[out], m, n, k, addr(status), stream_handle(cuda))
+    assert int(status.item()) == 0 and bool((c == float(k)).all())
